@@ -379,6 +379,26 @@ int sv_batchnorm_sync_bwd_apply(const void* x, const void* dy, const void* y_act
                                 int dbias_accumulate, int64_t rows, int C, int groups, void* workspace,
                                 size_t workspace_bytes, int dtype, sv_stream_t stream);
 
+/* ---- Group normalisation with a following activation.  No counterpart in the reference (its layers.BatchNormalization call
+ *      sites, unet.py:51-53, are where it can stand); the layer is tf.keras.layers.GroupNormalization (epsilon 1e-3).
+ *      x, y, dy, dx are [N, S, C] in the storage type `dtype`, S the product of the spatial extents; the C channels are
+ *      `groups` groups of C / groups consecutive ones, and each (sample, group) is normalised over its S * C / groups
+ *      elements: y = act((x - mean) * rstd * gamma + beta), rstd = 1 / sqrt(var + eps), var the biased variance.
+ *      C <= 4096.  N = 0 is allowed (the backward call then leaves zero parameter gradients, or the accumulated ones).
+ *  - save_mean / save_rstd [N, groups], f32: what the backward call needs; both may be NULL (inference).
+ *  - backward: dgamma / dbeta (+)= the sums over N and S, formed in a fixed order.  The activation's slope is recomputed
+ *    from x; at 0 it is that of the negative side.
+ *  - tensors need no alignment beyond their elements'; outputs must not overlap inputs.
+ *  workspace: sv_groupnorm_workspace_bytes, 16-byte aligned, for either direction. */
+size_t sv_groupnorm_workspace_bytes(int64_t N, int64_t S, int C, int groups);
+int sv_groupnorm_act_fwd(const void* x, const float* gamma, const float* beta, void* y, float* save_mean, float* save_rstd,
+                         int64_t N, int64_t S, int C, int groups, float eps, int act, float alpha, void* workspace,
+                         size_t workspace_bytes, int dtype, sv_stream_t stream);
+int sv_groupnorm_act_bwd(const void* x, const void* dy, const float* gamma, const float* beta, const float* save_mean,
+                         const float* save_rstd, void* dx, float* dgamma, float* dbeta, int accumulate, int64_t N,
+                         int64_t S, int C, int groups, int act, float alpha, void* workspace, size_t workspace_bytes,
+                         int dtype, sv_stream_t stream);
+
 /* ---- Concatenate on the channel axis (unet.py:144): y[r] = [a[r], b[r]] and its split backward */
 int sv_concat_channels_fwd(const void* a, const void* b, void* y, int64_t rows, int Ca, int Cb, int dtype,
                            sv_stream_t stream);
@@ -504,6 +524,47 @@ int sv_adam_keras_prepare(int64_t* step_state, float lr0, float beta1, float bet
                           float decay_rate, int staircase, sv_stream_t stream);
 int sv_adam_keras_apply(float* theta, float* grad, float* m, float* v, int64_t n, const int64_t* step_state,
                         float beta1, float beta2, float eps, float grad_scale, int zero_grad, sv_stream_t stream);
+
+/* ---- AdamW over a list of tensors in one launch (no counterpart in the reference, whose drivers build legacy Adam,
+ *      run_model.py:77-89; tf.keras.optimizers.AdamW with ExponentialDecay and global_clipnorm).  With t = count + 1, lr and
+ *      alpha as in sv_adam_keras_step, per element of every tensor:
+ *        g *= s;  m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2;  theta -= lr weight_decay theta;  theta -= alpha m/(sqrt(v)+eps)
+ *      s = grad_scale, or with clip_norm > 0 grad_scale * clip_norm / max(clip_norm, norm), norm = grad_scale * the 2-norm of all
+ *      gradients (one more launch; not finite: everything becomes NaN).
+ *  sv_adamw_tensor: one tensor.  n may be 0; weight_decay is its own; theta_bf16 may be NULL (a copy written with theta).
+ *      state_bits 32: m and v are float[n], m_exp / v_exp unused.
+ *      state_bits 8: m and v are uint8[n], m_exp / v_exp uint8[ceil(n / 256)], all zero at the start.  A block of 256 elements
+ *      shares the exponent byte e (255: a value of the block was not finite, the whole block reads as NaN).  A first
+ *      moment's code is sign, 4 exponent and 3 mantissa bits, a second moment's 5 exponent and 3 mantissa bits; it stands for the
+ *      float with the bits (code without sign) << 20, times 2^(e - 15) or 2^(e - 31).  e: the exponent field of the block's largest
+ *      magnitude once its mantissa is rounded up to 3 bits.  A value goes to the code above it if 16 random bits say so
+ *      (with the probability of its distance to the code below), a positive second moment to code 1 at least.  The bits of an
+ *      element are a hash of (seed, count, the element's position: 256 * the blocks of the tensors before it + its index).
+ *  A plan is a device copy of the host image that sv_adamw_plan_fill writes (sv_adamw_plan_bytes gives its size and
+ *      *n_chunks, both for sv_adamw_step); it holds the tensors' addresses.  No two buffers of a plan may overlap.
+ *  step_state: the 24 bytes of sv_adam_keras_step.  zero_grad: the gradients are cleared once read.
+ *  workspace: sv_adamw_workspace_bytes, 8-byte aligned; only read with clip_norm > 0.
+ *  sv_adamw_decode: out[i] = the value of codes[i] (second: of a second moment) for one tensor, or for several that lie back to
+ *      back in codes and exponents, each starting on a multiple of 256. */
+typedef struct sv_adamw_tensor {
+    float* theta;
+    float* grad;
+    void* m;
+    void* v;
+    uint8_t* m_exp;
+    uint8_t* v_exp;
+    void* theta_bf16;
+    int64_t n;
+    float weight_decay;
+    int32_t reserved;
+} sv_adamw_tensor;
+size_t sv_adamw_plan_bytes(const sv_adamw_tensor* tensors, int n_tensors, int64_t* n_chunks);
+int sv_adamw_plan_fill(const sv_adamw_tensor* tensors, int n_tensors, int state_bits, void* image, size_t image_bytes);
+size_t sv_adamw_workspace_bytes(void);
+int sv_adamw_step(const void* plan, int n_tensors, int64_t n_chunks, int state_bits, int64_t* step_state, double lr0,
+                  double beta1, double beta2, float eps, int decay_steps, double decay_rate, int staircase, float grad_scale,
+                  float clip_norm, uint64_t seed, int zero_grad, void* workspace, size_t workspace_bytes, sv_stream_t stream);
+int sv_adamw_decode(const uint8_t* codes, const uint8_t* exponents, float* out, int64_t n, int second, sv_stream_t stream);
 
 /* ---- deferred reductions (no reference counterpart; launch-count control for the backward pass of the GAN steps,
  *      run_context_encoder.py:225-260, run_unet.py:164-203).  Between _begin and _flush on one host thread, every

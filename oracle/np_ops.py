@@ -319,6 +319,40 @@ def batchnorm_train_bwd(x, gamma, dy, eps=1e-3):
 
 
 # --------------------------------------------------------------------------- dense / misc
+# ------------------------------------------------------------------------------------------- group norm + activation
+def act_slope(z, act, alpha=0.2):
+    """d act / d z from the pre-activation; at 0 the slope of the negative side."""
+    z = np.asarray(z, F64)
+    if act == "tanh":
+        return 1.0 / np.cosh(z) ** 2
+    return act_bwd_from_output(act_fwd(z, act, alpha), act, alpha)
+
+
+def group_norm(x, gamma, beta, groups, eps=1e-3, act=None, alpha=0.2):
+    """x [N, ..., C] -> (y, mean [N, G], rstd [N, G])."""
+    x = np.asarray(x, F64)
+    n, c = x.shape[0], x.shape[-1]
+    v = x.reshape(n, -1, groups, c // groups)
+    mean = v.mean(axis=(1, 3))
+    rstd = 1.0 / np.sqrt(v.var(axis=(1, 3)) + eps)
+    xhat = ((v - mean[:, None, :, None]) * rstd[:, None, :, None]).reshape(x.shape)
+    return act_fwd(xhat * gamma + beta, act, alpha), mean, rstd
+
+
+def group_norm_bwd(x, dy, gamma, beta, mean, rstd, groups, act=None, alpha=0.2):
+    """(dx, dgamma, dbeta) from the saved statistics."""
+    x, dy = np.asarray(x, F64), np.asarray(dy, F64)
+    n, c = x.shape[0], x.shape[-1]
+    shape = (n, -1, groups, c // groups)
+    mu, rs = mean.reshape(n, 1, groups, 1), rstd.reshape(n, 1, groups, 1)
+    xhat = (x.reshape(shape) - mu) * rs
+    flat = xhat.reshape(n, -1, c)
+    dz = dy.reshape(n, -1, c) * act_slope(flat * gamma + beta, act, alpha)
+    gz = (dz * gamma).reshape(shape)
+    dx = rs * (gz - gz.mean(axis=(1, 3), keepdims=True) - xhat * (gz * xhat).mean(axis=(1, 3), keepdims=True))
+    return dx.reshape(x.shape), (dz * flat).sum(axis=(0, 1)), dz.sum(axis=(0, 1))
+
+
 def dense(x, w, b=None):
     y = np.asarray(x, F64) @ np.asarray(w, F64)
     if b is not None:
@@ -456,6 +490,73 @@ def adam_keras_step(theta, g, m, v, it, lr, beta1=0.9, beta2=0.999, eps=1e-7):
 
 
 # --------------------------------------------------------------------------- initialisers
+def adamw_step(theta, g, m, v, it, lr, weight_decay, beta1=0.9, beta2=0.999, eps=1e-7):
+    """tf.keras.optimizers.AdamW: decay by lr * weight_decay, then the Keras-form Adam update."""
+    theta = np.asarray(theta, F64)
+    return adam_keras_step(theta - lr * weight_decay * theta, g, m, v, it, lr, beta1, beta2, eps)
+
+
+class Moments8:
+    """8-bit moments: blocks of 256 elements, codes of ``width`` exponent bits and 3 mantissa bits, one exponent byte a block
+    (255: not finite).  ``width`` 4: first moments (with a sign bit); 5: second moments."""
+
+    BLOCK = 256
+
+    @classmethod
+    def _blocks(cls, a):
+        a = np.asarray(a)
+        pad = -len(a) % cls.BLOCK
+        return np.concatenate([a, np.zeros(pad, a.dtype)]).reshape(-1, cls.BLOCK)
+
+    @classmethod
+    def random_bits(cls, n, first_block, it, seed):
+        """(16 bits of the first moment, 16 of the second) for elements 0..n of a tensor whose blocks start at
+        ``first_block``."""
+        key = mix64(mix64(it) ^ seed)
+        base = first_block * cls.BLOCK // 2
+        words = [mix64((base + p) ^ key) for p in range((n + 1) // 2)]
+        r = np.array([w >> s & 0xFFFFFFFF for w in words for s in (0, 32)], dtype=np.int64)[:n]
+        return r & 0xFFFF, r >> 16
+
+    @classmethod
+    def encode(cls, x, random16, width):
+        """(codes, exponents) of float32 values."""
+        x = cls._blocks(np.asarray(x, np.float32)).astype(F64)
+        r = cls._blocks(random16)
+        big = np.abs(x).max(axis=1)
+        finite = np.isfinite(big)
+        x = np.where(finite[:, None], x, 0.0)
+        frac, e = np.frexp(np.where(finite, big, 0.0))
+        up = np.ceil(frac * 16) / 16  # mantissa rounded up to 3 bits (the leading one is the fourth)
+        field = np.where(big == 0, 0, np.where(up == 1.0, e + 1, e) + 126)  # exponent field of a float32
+        field = np.maximum(field, 0)  # a block of float32 denormals
+        finite &= field < 255
+        top = (1 << width) - 1
+        scaled = np.abs(x) * 2.0 ** (top - np.where(finite, field, 0).astype(F64))[:, None]  # field `top` is the largest
+        scaled = scaled.astype(np.float32).astype(F64)
+        own = np.maximum(np.where(scaled > 0, np.frexp(scaled)[1], -125), -125)  # exponent of the value's binade; below the last: the denormals' step
+        step = 2.0 ** (own - 4.0)
+        code = np.floor(scaled / step + r / 65536.0)  # in steps of its own binade: 8..16, or 0..8 among the denormals
+        code = np.where(own == -125, code, code + 8.0 * (own + 125))
+        if width == 5:
+            code = np.where((x > 0) & (code == 0), 1, code)
+        code = code.astype(np.int64)
+        if width == 4:
+            code |= np.signbit(x).astype(np.int64) << 7
+        code = np.where(finite[:, None], code, 0)
+        return code.reshape(-1)[:len(random16)].astype(np.uint8), np.where(finite, field, 255).astype(np.uint8)
+
+    @classmethod
+    def decode(cls, codes, exponents, width):
+        code = cls._blocks(np.asarray(codes)).astype(np.int64)
+        size, sign = code & ((8 << width) - 1), np.where((code >> 7 & 1) & (width == 4), -1.0, 1.0)
+        field = size >> 3
+        value = np.where(field == 0, (size & 7) * 2.0 ** -129, (8 + (size & 7)) * 2.0 ** (field - 130.0))
+        value = sign * value * 2.0 ** (exponents.astype(F64)[:, None] - ((1 << width) - 1))
+        value = np.where(exponents[:, None] == 255, np.nan, value)
+        return value.reshape(-1)[:len(codes)].astype(np.float32)
+
+
 def glorot_uniform_limit(shape):
     """keras glorot_uniform: fans = receptive field * channels."""
     if len(shape) == 2:

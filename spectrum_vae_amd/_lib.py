@@ -72,6 +72,14 @@ class DgradJob(C.Structure):
                 ("dx", C.c_void_p), ("act", C.c_int32), ("alpha", C.c_float)]
 
 
+class AdamWTensor(C.Structure):
+    """Mirror of ``sv_adamw_tensor``."""
+
+    _fields_ = [("theta", C.c_void_p), ("grad", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p), ("m_exp", C.c_void_p),
+                ("v_exp", C.c_void_p), ("theta_bf16", C.c_void_p), ("n", C.c_int64), ("weight_decay", C.c_float),
+                ("reserved", C.c_int32)]
+
+
 _p, _i, _f, _i64, _u64, _sz = C.c_void_p, C.c_int, C.c_float, C.c_int64, C.c_uint64, C.c_size_t
 _g = C.POINTER(ConvGeom)
 
@@ -136,6 +144,9 @@ SIGNATURES = {
                                          _sz, _i, _p]),
     "sv_batchnorm_act_bwd": (_i, [_p, _p, _p, _i, _f, _p, _p, _p, _p, _p, _p, _i, _i, _f, _p, _i, _i64, _i, _i, _p, _sz,
                                   _i, _p]),
+    "sv_groupnorm_workspace_bytes": (_sz, [_i64, _i64, _i, _i]),
+    "sv_groupnorm_act_fwd": (_i, [_p] * 6 + [_i64, _i64, _i, _i, _f, _i, _f, _p, _sz, _i, _p]),
+    "sv_groupnorm_act_bwd": (_i, [_p] * 9 + [_i, _i64, _i64, _i, _i, _i, _f, _p, _sz, _i, _p]),
     "sv_concat_channels_fwd": (_i, [_p, _p, _p, _i64, _i, _i, _i, _p]),
     "sv_concat_channels_bwd": (_i, [_p, _p, _p, _i64, _i, _i, _i, _p]),
     "sv_dense_fwd": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _f, _i, _p]),
@@ -166,6 +177,12 @@ SIGNATURES = {
     "sv_scalar_program": (_i, [_i, _p, _p, _p, _p, _p, _p]),
     "sv_adam_keras_prepare": (_i, [_p, _f, _f, _f, _i, _f, _i, _p]),
     "sv_adam_keras_apply": (_i, [_p, _p, _p, _p, _i64, _p, _f, _f, _f, _f, _i, _p]),
+    "sv_adamw_plan_bytes": (_sz, [C.POINTER(AdamWTensor), _i, C.POINTER(C.c_int64)]),
+    "sv_adamw_plan_fill": (_i, [C.POINTER(AdamWTensor), _i, _i, _p, _sz]),
+    "sv_adamw_workspace_bytes": (_sz, []),
+    "sv_adamw_step": (_i, [_p, _i, _i64, _i, _p, C.c_double, C.c_double, C.c_double, _f, _i, C.c_double, _i, _f, _f, _u64, _i,
+                           _p, _sz, _p]),
+    "sv_adamw_decode": (_i, [_p, _p, _p, _i64, _i, _p]),
     "sv_gather_rows": (_i, [_p, _i, _p, _p, _i64, _i64, _p]),
     "sv_conv2d_masked_supported": (_i, [_g]),
     "sv_conv2d_fwd_masked": (_i, [_g, _p, _p, _p, _p, _p, _i, _f, _p, _sz, _i, _p]),

@@ -651,7 +651,8 @@ class Model(Layer):
             main.wait_event(zeroed)
         # without a reducer (which needs the summed gradients in the flat buffer) the optimizer launch may take the
         # kernel gradients as slabs of partial sums
-        self._slabs_wanted = side is None and self._reducer is None and hasattr(self.optimizer, "apply_model")
+        self._slabs_wanted = (side is None and self._reducer is None and hasattr(self.optimizer, "apply_model")
+                              and getattr(self.optimizer, "takes_slabs", True))
         self._pending_slabs = None
         try:
             self.backward_raw(b["dpred"], -1, need_dx=False)

@@ -816,12 +816,68 @@ class BatchNormalization(Layer):
         return dx
 
 
+class GroupNormalization(Layer):
+    """tf.keras.layers.GroupNormalization on the channel axis (no reference counterpart; stands where the reference's models
+    have BatchNormalization): every sample is normalised by itself, over its spatial extents and the channels of a group, so
+    training and inference are the same function and neither the batch size nor data-parallel replicas enter.
+    ``groups=-1``: one group per channel."""
+
+    def __init__(self, groups=32, epsilon=1e-3, name=None):
+        super().__init__(name)
+        self.groups = int(groups)
+        self.epsilon = float(epsilon)
+
+    fused_act = None  # (act, alpha) of the activation layer that follows: applied in this layer's launches (Sequential)
+
+    def _build(self, in_shape):
+        c = in_shape[-1]
+        if self.groups == -1:
+            self.groups = c
+        if self.groups < 1 or c % self.groups:
+            raise ValueError(f"{self.name}: {c} channels do not split into {self.groups} groups")
+        self.gamma = self.add_weight("gamma", (c,), "ones")
+        self.beta = self.add_weight("beta", (c,), "zeros")
+        return in_shape
+
+    def _scratch(self, ctx, x):
+        n, c = x.shape[0], x.shape[-1]
+        return ctx.pool.workspace(ops.groupnorm_workspace(n, x.numel() // max(n * c, 1), c, self.groups))
+
+    def forward(self, ctx, x):
+        y = ctx.buf(self, "y", tuple(x.shape))
+        act, alpha = self.fused_act if self.fused_act is not None else (None, 0.0)
+        mean = rstd = None
+        if ctx.training:
+            mean = ctx.buf(self, "mean", (x.shape[0], self.groups), torch.float32)
+            rstd = ctx.buf(self, "rstd", (x.shape[0], self.groups), torch.float32)
+            # names of their own: a statistics group's view of the call (CallCtx.group_view) cuts them by sample
+            ctx.saved[id(self)] = {"x": x, "sample_mean": mean, "sample_rstd": rstd}
+        ops.groupnorm_act_fwd(x, self.gamma.data, self.beta.data, y, mean, rstd, self.groups, self.epsilon, act, alpha,
+                              self._scratch(ctx, x))
+        return y
+
+    def backward(self, ctx, dy, need_dx=True):
+        s = ctx.saved[id(self)]
+        x = s["x"]
+        c = self.input_shape_[-1]
+        dx = ctx.buf(self, "dx", tuple(x.shape))
+        if ctx.param_grads:
+            dg, db, acc = self.gamma.grad, self.beta.grad, True
+        else:
+            dg, db, acc = (ctx.buf(self, "dg_scratch", (c,), torch.float32),
+                           ctx.buf(self, "db_scratch", (c,), torch.float32), False)
+        act, alpha = self.fused_act if self.fused_act is not None else (None, 0.0)
+        ops.groupnorm_act_bwd(x, dy, self.gamma.data, self.beta.data, s["sample_mean"], s["sample_rstd"], dx, dg, db, acc,
+                              self.groups, act, alpha, self._scratch(ctx, x))
+        return dx
+
+
 class Activation(Layer):
     def __init__(self, activation, name=None):
         super().__init__(name)
         self.act, self.alpha = _act_name(activation)
 
-    folded = False  # applied inside the BatchNormalization in front of it (set by Sequential's planner)
+    folded = False  # applied inside the normalisation layer in front of it (set by Sequential's planner)
 
     def forward(self, ctx, x):
         if self.act is None or self.folded:
@@ -1029,12 +1085,14 @@ class Sequential(Layer):
             shape = l.build(shape)
         if self.fuse and os.environ.get("SPECTRUM_BN_FUSE", "1") != "0":
             for i, l in enumerate(self.layers):
-                if not isinstance(l, BatchNormalization):
+                if not isinstance(l, (BatchNormalization, GroupNormalization)):
                     continue
                 nxt = self.layers[i + 1] if i + 1 < len(self.layers) else None
                 if type(nxt) in (Activation, LeakyReLU) and nxt.act is not None:
-                    l.fused_act = (nxt.act, nxt.alpha)  # BatchNormalization -> activation in one launch (unet.py:51-53)
+                    l.fused_act = (nxt.act, nxt.alpha)  # normalisation -> activation in one launch (unet.py:51-53)
                     nxt.folded = True
+                if not isinstance(l, BatchNormalization):
+                    continue
                 prv = self.layers[i - 1] if i > 0 else None
                 if isinstance(prv, _ConvBase) and prv.act is not None:
                     l.prev_conv = prv  # conv(activation) -> BatchNormalization (context_encoder.py:61-64), backward side

@@ -12,7 +12,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import ACT, BF16, F32, BatchRows, ConvGeom, DgradJob, GradSlabs, NetLayer, WgradBatchJob, WgradJob, check, lib
+from ._lib import ACT, BF16, F32, AdamWTensor, BatchRows, ConvGeom, DgradJob, GradSlabs, NetLayer, WgradBatchJob, WgradJob, check, lib
 
 
 def set_option(name: str, value: int):
@@ -529,6 +529,77 @@ def batchnorm_sync_bwd_apply(x, dy, y_act, act_out, alpha_out: float, gamma, mea
           "sv_batchnorm_sync_bwd_apply")
 
 
+class _on:
+    """``with _on(x, ...) as stream``: the device all these tensors are on becomes the current one for the block; ``stream``
+    is its current stream."""
+
+    def __init__(self, first, *rest):
+        dev = first.device
+        for t in rest:
+            if t is not None and t.device != dev:
+                raise ValueError(f"tensors on {dev} and {t.device}: a launch takes tensors of one device")
+        if not first.is_cuda:
+            raise _lib.SpectrumHipError(f"tensor is on {dev}: the HIP path needs device tensors (no CPU fallback)")
+        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return _stream()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def groupnorm_workspace(n: int, s: int, c: int, groups: int) -> int:
+    """Scratch bytes of ``groupnorm_act_fwd`` / ``groupnorm_act_bwd`` on [n, s, c] activations (s: product of the spatial
+    extents)."""
+    return int(lib.sv_groupnorm_workspace_bytes(n, s, c, groups))
+
+
+def _groupnorm_extents(x, like, gamma, beta, mean, rstd, groups: int):
+    if x.dim() < 2 or like.shape != x.shape:
+        raise ValueError(f"groupnorm: [N, ..., C] tensors of one shape, not {tuple(x.shape)} and {tuple(like.shape)}")
+    n, c = x.shape[0], x.shape[-1]
+    s = 1
+    for d in x.shape[1:-1]:
+        s *= d
+    if groups < 1 or c % groups:
+        raise ValueError(f"groupnorm: {c} channels do not split into {groups} groups")
+    if gamma.numel() != c or beta.numel() != c:
+        raise ValueError(f"groupnorm: gamma / beta must have the {c} channels' size")
+    if (mean is None) != (rstd is None):
+        raise ValueError("groupnorm: saved mean and rstd go together")
+    if mean is not None and (mean.numel() != n * groups or rstd.numel() != n * groups):
+        raise ValueError("groupnorm: saved statistics must be [N][groups]")
+    return n, s, c
+
+
+def groupnorm_act_fwd(x, gamma, beta, y, save_mean, save_rstd, groups: int, eps: float, act, alpha: float, ws):
+    """y = act((x - mean) * rstd * gamma + beta), mean and rstd over each sample's channel groups; x, y [N, ..., C] float32 or
+    bfloat16, everything else float32.  save_mean / save_rstd [N, groups]: for the backward call; both may be None."""
+    n, s, c = _groupnorm_extents(x, y, gamma, beta, save_mean, save_rstd, groups)
+    with _on(x, gamma, beta, y, save_mean, save_rstd, ws) as stream:
+        check(lib.sv_groupnorm_act_fwd(_aptr(x), _ptr(gamma), _ptr(beta), _aptr(y, x, "y"), _ptr(save_mean), _ptr(save_rstd),
+                                       n, s, c, groups, eps, ACT[act], alpha, *_ws_args(ws), _dt(x), stream),
+              "sv_groupnorm_act_fwd")
+
+
+def groupnorm_act_bwd(x, dy, gamma, beta, save_mean, save_rstd, dx, dgamma, dbeta, accumulate: bool, groups: int, act,
+                      alpha: float, ws):
+    """Backward of ``groupnorm_act_fwd`` from its input (its output is not needed): dx, and dgamma / dbeta (+)= their sums."""
+    if save_mean is None or dx.shape != x.shape:
+        raise ValueError("groupnorm: the backward call needs the saved statistics and dx of x's shape")
+    n, s, c = _groupnorm_extents(x, dy, gamma, beta, save_mean, save_rstd, groups)
+    if dgamma.numel() != c or dbeta.numel() != c:
+        raise ValueError(f"groupnorm: dgamma / dbeta must have the {c} channels' size")
+    with _on(x, dy, gamma, beta, save_mean, save_rstd, dx, dgamma, dbeta, ws) as stream:
+        check(lib.sv_groupnorm_act_bwd(_aptr(x), _aptr(dy, x, "dy"), _ptr(gamma), _ptr(beta), _ptr(save_mean), _ptr(save_rstd),
+                                       _aptr(dx, x, "dx"), _ptr(dgamma), _ptr(dbeta), int(accumulate), n, s, c, groups,
+                                       ACT[act], alpha, *_ws_args(ws), _dt(x), stream), "sv_groupnorm_act_bwd")
+
+
 def concat_channels_fwd(a, b, y, rows, ca, cb):
     check(lib.sv_concat_channels_fwd(_aptr(a), _aptr(b, a, "b"), _aptr(y, a, "y"), rows, ca, cb, _dt(a), _stream()),
           "sv_concat_channels_fwd")
@@ -679,6 +750,86 @@ def adam_apply(theta, grad, m, v, state, beta1, beta2, eps, grad_scale=1.0, zero
         raise ValueError("adam: buffer sizes differ")
     check(lib.sv_adam_keras_apply(_ptr(theta), _ptr(grad), _ptr(m), _ptr(v), theta.numel(), _ptr(state, torch.int64),
                                   beta1, beta2, eps, grad_scale, int(zero_grad), _stream()), "sv_adam_keras_apply")
+
+
+ADAMW_BLOCK = 256  # elements of one tensor that share an exponent byte of 8-bit moments
+
+
+class AdamWPlan:
+    """The tensors of an ``adamw_step``: equally long lists of parameters and gradients (float32), first and second moments
+    (all float32, or all uint8 codes with uint8 exponents ``m_exp`` / ``v_exp`` of one byte per 256 elements; zero-filled
+    moments are the start in either form), one weight decay each (or one for all), optionally bfloat16 copies
+    ``params_lp`` that the step refreshes.  The plan keeps the tensors; its table of their addresses is made once and lies on
+    their device."""
+
+    def __init__(self, params, grads, m, v, weight_decay, m_exp=None, v_exp=None, params_lp=None):
+        params = list(params)
+        if not params:
+            raise ValueError("adamw: an empty list of tensors")
+        decay = [float(weight_decay)] * len(params) if isinstance(weight_decay, (int, float)) else [float(w) for w in weight_decay]
+        cols = {"grads": list(grads), "m": list(m), "v": list(v), "weight_decay": decay}
+        if (m_exp is None) != (v_exp is None):
+            raise ValueError("adamw: m_exp and v_exp go together")
+        for name, col in (("m_exp", m_exp), ("v_exp", v_exp), ("params_lp", params_lp)):
+            cols[name] = list(col) if col is not None else [None] * len(params)
+        for name, col in cols.items():
+            if len(col) != len(params):
+                raise ValueError(f"adamw: {len(params)} parameters and {len(col)} of {name}")
+        self.state_bits = 32 if m_exp is None else 8
+        state = torch.float32 if m_exp is None else torch.uint8
+        self.device = params[0].device
+        table = (AdamWTensor * len(params))()
+        for i, (t, p) in enumerate(zip(table, params)):
+            g, mi, vi, me, ve, lp = (cols[k][i] for k in ("grads", "m", "v", "m_exp", "v_exp", "params_lp"))
+            n = p.numel()
+            if any(q is not None and q.numel() != n for q in (g, mi, vi, lp)):
+                raise ValueError(f"adamw: buffer sizes of tensor {i} differ")
+            if any(q is not None and q.numel() != -(-n // ADAMW_BLOCK) for q in (me, ve)):
+                raise ValueError(f"adamw: tensor {i} needs one exponent per {ADAMW_BLOCK} elements")
+            if any(q is not None and q.device != self.device for q in (p, g, mi, vi, me, ve, lp)):
+                raise ValueError(f"adamw: tensor {i} is on another device than the first")
+            t.theta, t.grad = _ptr(p, name=f"parameter {i}"), _ptr(g, name=f"gradient {i}")
+            t.m, t.v = _ptr(mi, state, f"m {i}"), _ptr(vi, state, f"v {i}")
+            t.m_exp, t.v_exp = _ptr(me, torch.uint8, f"m_exp {i}"), _ptr(ve, torch.uint8, f"v_exp {i}")
+            t.theta_bf16 = _ptr(lp, torch.bfloat16, f"params_lp {i}")
+            t.n, t.weight_decay, t.reserved = n, cols["weight_decay"][i], 0
+        chunks = C.c_int64(0)
+        nbytes = int(lib.sv_adamw_plan_bytes(table, len(params), C.byref(chunks)))
+        image = torch.empty(max(nbytes, 1), dtype=torch.uint8)
+        check(lib.sv_adamw_plan_fill(table, len(params), self.state_bits, image.data_ptr(), nbytes), "sv_adamw_plan_fill")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("adamw: a plan cannot be made while a graph is being recorded")
+        self.n_tensors, self.n_chunks = len(params), int(chunks.value)
+        self.elements = sum(p.numel() for p in params)
+        self._keep = (params, cols)  # the table holds their addresses
+        self._image = image.to(self.device)
+        self._ws = torch.empty(int(lib.sv_adamw_workspace_bytes()), dtype=torch.uint8, device=self.device)
+
+
+def adamw_step(plan: AdamWPlan, state, lr0, beta1, beta2, eps, decay_steps=0, decay_rate=1.0, staircase=False, grad_scale=1.0,
+               clip_norm=0.0, seed=0, zero_grad=False):
+    """One AdamW update of every tensor of ``plan``: schedule, decoupled weight decay and update in one launch.  ``state``:
+    int64[3] on the device, zero-filled at the start, with the update count (the layout ``adam_step`` keeps).
+    ``clip_norm`` > 0: gradients are scaled by clip_norm / max(clip_norm, their global 2-norm) (one more launch).  ``seed``:
+    of the random bits that round 8-bit moments."""
+    if state.numel() < 3:
+        raise ValueError("adamw: the step state is int64[3]")
+    with _on(plan._image, state) as stream:
+        check(lib.sv_adamw_step(plan._image.data_ptr(), plan.n_tensors, plan.n_chunks, plan.state_bits,
+                                _ptr(state, torch.int64), lr0, beta1, beta2, eps, int(decay_steps or 0), decay_rate,
+                                int(staircase), grad_scale, clip_norm, seed, int(zero_grad), plan._ws.data_ptr(),
+                                plan._ws.numel(), stream), "sv_adamw_step")
+
+
+def adamw_decode(codes, exponents, out, second: bool):
+    """float32 values of 8-bit moments (``second``: second moments) of one tensor, or of several laid back to back with each on
+    a multiple of 256 elements."""
+    n = codes.numel()
+    if out.numel() != n or exponents.numel() != -(-n // ADAMW_BLOCK):
+        raise ValueError("adamw_decode: sizes differ")
+    with _on(codes, exponents, out) as stream:
+        check(lib.sv_adamw_decode(_ptr(codes, torch.uint8), _ptr(exponents, torch.uint8), _ptr(out), n, int(bool(second)),
+                                  stream), "sv_adamw_decode")
 
 
 # --------------------------------------------------------------------------- batching helpers

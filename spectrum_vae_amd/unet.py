@@ -16,8 +16,8 @@ import torch
 from . import global_vars, ops
 from .losses import to_device_f32
 from .model import Model
-from .nn import (BatchNormalization, CallCtx, Conv2D, Conv2DTranspose, Flatten, Layer, LeakyReLU, Sequential,
-                 as_dtensor, default_device)
+from .nn import (BatchNormalization, CallCtx, Conv2D, Conv2DTranspose, Flatten, GroupNormalization, Layer, LeakyReLU,
+                 Sequential, as_dtensor, default_device)
 
 # unet.py:13-26
 final_width = 4
@@ -30,13 +30,16 @@ for _fi in range(1, n_filters):
 
 
 def convolution(n_filters: int, kernel: Tuple[int, int], stride: Tuple[int, int], apply_batchnorm: bool = True,
-                padding: str = "same") -> Sequential:
-    """unet.py:29-55: Conv2D(no bias, N(0, 0.02) init) -> BatchNorm -> LeakyReLU(0.2)."""
+                padding: str = "same", normalization: str = "batch", groups: int = 8) -> Sequential:
+    """unet.py:29-55: Conv2D(no bias, N(0, 0.02) init) -> BatchNorm -> LeakyReLU(0.2).  ``normalization="group"`` (not the
+    reference's): GroupNormalization over ``groups`` channel groups in the place of BatchNorm."""
+    if normalization not in ("batch", "group"):
+        raise ValueError(f"normalization {normalization!r}: 'batch' or 'group'")
     block = Sequential(name=None)
     block.add(Conv2D(n_filters, kernel, strides=stride, padding=padding, kernel_initializer="normal0.02",
                      use_bias=False))
     if apply_batchnorm:
-        block.add(BatchNormalization())
+        block.add(BatchNormalization() if normalization == "batch" else GroupNormalization(groups))
     block.add(LeakyReLU(0.2))
     return block
 
@@ -59,11 +62,12 @@ class ContextEncoder(Model):
     (so it is re-initialised on every eager call); here it is constructed once."""
 
     def __init__(self, kernel: Tuple[int, int] = (2, 2), stride: Tuple[int, int] = (2, 2),
-                 latent_dimensions: int = 128, input_shape=None):
+                 latent_dimensions: int = 128, input_shape=None, normalization: str = "batch"):
         super().__init__(name="unet")
         self.kernel, self.stride, self.latent_dimensions = kernel, stride, latent_dimensions
         self.declared_input_shape = input_shape
-        self.encoder_stack: List[Sequential] = [convolution(64, kernel, stride) for _ in range(4)]
+        self.encoder_stack: List[Sequential] = [convolution(64, kernel, stride, normalization=normalization)
+                                               for _ in range(4)]
         self.decoder_stack: List[Sequential] = [upconvolution(64, kernel, stride) for _ in range(3)]
         self.final_conv = Conv2DTranspose(global_vars.OUTPUT_CHANNELS, kernel, strides=stride, padding="same",
                                           kernel_initializer="normal0.02", activation="tanh")
@@ -121,8 +125,8 @@ class Generator(ContextEncoder):
     """What ``run_unet.py:33,276`` calls ``unet.Generator``: the skip-connected U-Net above
     (INPUT_CHANNELS in, OUTPUT_CHANNELS out).  No definition exists in the reference."""
 
-    def __init__(self, input_shape=None, kernel=(2, 2), stride=(2, 2)):
-        super().__init__(kernel=kernel, stride=stride, input_shape=input_shape)
+    def __init__(self, input_shape=None, kernel=(2, 2), stride=(2, 2), normalization: str = "batch"):
+        super().__init__(kernel=kernel, stride=stride, input_shape=input_shape, normalization=normalization)
         self.name = "generator"
 
 
@@ -133,13 +137,13 @@ class Discriminator(Model):
     The reference's class of this name cannot be constructed (unet.py:177), so this structure is the
     build's own (a pix2pix-style patch discriminator collapsed to one logit)."""
 
-    def __init__(self, kernel_size: int = 4):
+    def __init__(self, kernel_size: int = 4, normalization: str = "batch"):
         super().__init__(name="unet_discriminator")
         k = (kernel_size, kernel_size)
         self.blocks: List[Sequential] = [
             convolution(64, k, (2, 2), apply_batchnorm=False),
-            convolution(128, k, (2, 2)),
-            convolution(256, k, (2, 2)),
+            convolution(128, k, (2, 2), normalization=normalization),
+            convolution(256, k, (2, 2), normalization=normalization),
         ]
         self.head = Sequential([Conv2D(1, k, strides=(1, 1), padding="valid", kernel_initializer="normal0.02"),
                                 Flatten()], name="head")
