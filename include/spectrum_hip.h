@@ -561,9 +561,9 @@ typedef struct sv_adamw_tensor {
 size_t sv_adamw_plan_bytes(const sv_adamw_tensor* tensors, int n_tensors, int64_t* n_chunks);
 int sv_adamw_plan_fill(const sv_adamw_tensor* tensors, int n_tensors, int state_bits, void* image, size_t image_bytes);
 size_t sv_adamw_workspace_bytes(void);
-int sv_adamw_step(const void* plan, int n_tensors, int64_t n_chunks, int state_bits, int64_t* step_state, double lr0,
-                  double beta1, double beta2, float eps, int decay_steps, double decay_rate, int staircase, float grad_scale,
-                  float clip_norm, uint64_t seed, int zero_grad, void* workspace, size_t workspace_bytes, sv_stream_t stream);
+int sv_adamw_step(const void* plan, int64_t n_chunks, int state_bits, int64_t* step_state, double lr0, double beta1, double beta2,
+                  float eps, int decay_steps, double decay_rate, int staircase, float grad_scale, float clip_norm, uint64_t seed,
+                  int zero_grad, void* workspace, size_t workspace_bytes, sv_stream_t stream);
 int sv_adamw_decode(const uint8_t* codes, const uint8_t* exponents, float* out, int64_t n, int second, sv_stream_t stream);
 
 /* ---- deferred reductions (no reference counterpart; launch-count control for the backward pass of the GAN steps,

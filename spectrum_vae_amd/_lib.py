@@ -180,7 +180,7 @@ SIGNATURES = {
     "sv_adamw_plan_bytes": (_sz, [C.POINTER(AdamWTensor), _i, C.POINTER(C.c_int64)]),
     "sv_adamw_plan_fill": (_i, [C.POINTER(AdamWTensor), _i, _i, _p, _sz]),
     "sv_adamw_workspace_bytes": (_sz, []),
-    "sv_adamw_step": (_i, [_p, _i, _i64, _i, _p, C.c_double, C.c_double, C.c_double, _f, _i, C.c_double, _i, _f, _f, _u64, _i,
+    "sv_adamw_step": (_i, [_p, _i64, _i, _p, C.c_double, C.c_double, C.c_double, _f, _i, C.c_double, _i, _f, _f, _u64, _i,
                            _p, _sz, _p]),
     "sv_adamw_decode": (_i, [_p, _p, _p, _i64, _i, _p]),
     "sv_gather_rows": (_i, [_p, _i, _p, _p, _i64, _i64, _p]),

@@ -26,7 +26,9 @@ constexpr int kBlock = 256;        // elements of an 8-bit block
 constexpr int kChunk = 4096;       // elements of one tensor that a workgroup updates at a time
 constexpr int kNormParts = 1024;   // most workgroups (partial sums) of the norm launch
 
-struct Tensor {  // one entry of the device table
+// One entry of the plan on the device: up to kChunk consecutive elements of one tensor.  Pointers are to the chunk's own first
+// element, so a workgroup gets to its data through a single dependent load.
+struct Chunk {
     float* theta;
     float* grad;
     void* m;
@@ -34,18 +36,14 @@ struct Tensor {  // one entry of the device table
     uint8_t* m_exp;
     uint8_t* v_exp;
     __bf16* theta_lp;
-    int64_t n;
-    int64_t first_block;  // of its 8-bit blocks among all tensors' (the position in the random stream)
+    int64_t block;  // its first 8-bit block's number among those of all tensors (the position in the random stream)
+    int32_t n;
     float decay;
-    int32_t vec;          // every pointer takes 4-element accesses
+    int32_t vec;    // every pointer takes 4-element accesses
+    int32_t pad;
 };
-struct Chunk {
-    int32_t tensor, index;
-};
-// device image: Tensor[n_tensors], Chunk[n_chunks]
 
 struct StepArgs {
-    const Tensor* tensors;
     const Chunk* chunks;
     int64_t n_chunks;
     int64_t* state;
@@ -84,6 +82,7 @@ __device__ __forceinline__ uint32_t second_code(float v, int e, uint32_t random1
     return c == 0u && v > 0.f ? 1u : c;
 }
 
+// Root and quotient are the hardware's (1 ulp each): they only enter theta's step.
 __device__ __forceinline__ void update(float& th, float& m, float& v, float g, const StepArgs& a, float scale, float alpha,
                                        float lr_decay) {
 #pragma clang fp contract(off)
@@ -91,7 +90,7 @@ __device__ __forceinline__ void update(float& th, float& m, float& v, float g, c
     m = a.beta1 * m + a.one_minus_beta1 * gs;
     v = a.beta2 * v + a.one_minus_beta2 * (gs * gs);
     th = th - lr_decay * th;
-    th = th - (alpha * m) / (sqrtf(v) + a.eps);
+    th = th - (alpha * m) * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v) + a.eps);
 }
 
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
@@ -103,19 +102,23 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
     return v;
 }
 
-// Partial sums of squares of the gradients, one a workgroup, in f64.
-__global__ __launch_bounds__(256) void grad_norm_k(const Tensor* __restrict__ tensors, const Chunk* __restrict__ chunks,
-                                                    int64_t n_chunks, double* __restrict__ parts) {
+// Partial sums of squares of the gradients, one a workgroup: 16 squares a thread in f32, everything else in f64.
+__global__ __launch_bounds__(256) void grad_norm_k(const Chunk* __restrict__ chunks, int64_t n_chunks, double* __restrict__ parts) {
     __shared__ double red[4];
     double sum = 0.0;
     for (int64_t k = blockIdx.x; k < n_chunks; k += gridDim.x) {
-        const Chunk ck = chunks[k];
-        const Tensor& t = tensors[ck.tensor];
-        const int64_t i0 = (int64_t)ck.index * kChunk;
-        const int n = (int)(t.n - i0 < kChunk ? t.n - i0 : kChunk);
-        const float* g = t.grad + i0;
+        const float* g = chunks[k].grad;
+        const int n = chunks[k].n;
         float s = 0.f;
-        for (int i = threadIdx.x; i < n; i += 256) s = fmaf(g[i], g[i], s);
+        if (chunks[k].vec && n == kChunk) {
+            float4 q[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) q[u] = reinterpret_cast<const float4*>(g)[threadIdx.x + 256 * u];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) s = fmaf(q[u].x, q[u].x, fmaf(q[u].y, q[u].y, fmaf(q[u].z, q[u].z, fmaf(q[u].w, q[u].w, s))));
+        } else {
+            for (int i = threadIdx.x; i < n; i += 256) s = fmaf(g[i], g[i], s);
+        }
         sum += (double)s;
     }
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
@@ -124,113 +127,166 @@ __global__ __launch_bounds__(256) void grad_norm_k(const Tensor* __restrict__ te
     if (threadIdx.x == 0) parts[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
 }
 
-// A wave takes blocks of 256 elements, four a lane.
+// Four consecutive elements of a lane: VEC as one access, else the first `mine` one by one (the others read as 0).
+template <typename E, typename Q>
+__device__ __forceinline__ void load4(const E* p, bool vec, int mine, E (&out)[4]) {
+    if (vec) {
+        const Q q = *reinterpret_cast<const Q*>(p);
+        __builtin_memcpy(out, &q, sizeof(q));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[e] = e < mine ? p[e] : (E)0;
+    }
+}
+template <typename E, typename Q>
+__device__ __forceinline__ void store4(E* p, bool vec, int mine, const E (&in)[4]) {
+    if (vec) {
+        Q q;
+        __builtin_memcpy(&q, in, sizeof(q));
+        *reinterpret_cast<Q*>(p) = q;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < mine) p[e] = in[e];
+    }
+}
+
+// What a lane holds of a block of 256 elements.
+template <int BITS>
+struct Held {
+    float th[4], g[4], m[4], v[4];
+    uint8_t mc[4], vc[4];
+    int me, ve, mine;
+    bool vec;
+
+    __device__ __forceinline__ void load(const Chunk& c, int b, int lane) {
+        const int i = b * kBlock + 4 * lane;
+        mine = c.n - i >= 4 ? 4 : c.n - i > 0 ? c.n - i : 0;
+        vec = c.vec && c.n - b * kBlock >= kBlock;  // the same for the whole wave
+        load4<float, float4>(c.theta + i, vec, mine, th);
+        load4<float, float4>(c.grad + i, vec, mine, g);
+        if (BITS == 8) {
+            me = c.m_exp[b];
+            ve = c.v_exp[b];
+            load4<uint8_t, uint32_t>((const uint8_t*)c.m + i, vec, mine, mc);
+            load4<uint8_t, uint32_t>((const uint8_t*)c.v + i, vec, mine, vc);
+        } else {
+            load4<float, float4>((const float*)c.m + i, vec, mine, m);
+            load4<float, float4>((const float*)c.v + i, vec, mine, v);
+        }
+    }
+
+    __device__ __forceinline__ void step(const Chunk& c, int b, int lane, const StepArgs& a, float scale, float alpha,
+                                         float lr_decay, uint64_t key) {
+        const int i = b * kBlock + 4 * lane;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (BITS == 8) {
+                m[e] = first_value(mc[e], me);
+                v[e] = second_value(vc[e], ve);
+            }
+            update(th[e], m[e], v[e], g[e], a, scale, alpha, lr_decay);
+        }
+        if (BITS == 8) {
+            uint32_t ml = 0, vl = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t mb = e < mine ? __float_as_uint(m[e]) & 0x7fffffffu : 0u;
+                const uint32_t vb = e < mine ? __float_as_uint(v[e]) & 0x7fffffffu : 0u;
+                ml = mb > ml ? mb : ml;
+                vl = vb > vl ? vb : vl;
+            }
+            me = block_exponent(wave_max(ml));
+            ve = block_exponent(wave_max(vl));
+            const uint64_t pair = (uint64_t)((c.block + b) * (kBlock / 2) + 2 * lane);
+            const uint64_t h0 = mix64(pair ^ key), h1 = mix64((pair + 1) ^ key);
+            const uint32_t r[4] = {(uint32_t)h0, (uint32_t)(h0 >> 32), (uint32_t)h1, (uint32_t)(h1 >> 32)};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                mc[e] = (uint8_t)first_code(m[e], me, r[e] & 0xffffu);
+                vc[e] = (uint8_t)second_code(v[e], ve, r[e] >> 16);
+            }
+            store4<uint8_t, uint32_t>((uint8_t*)c.m + i, vec, mine, mc);
+            store4<uint8_t, uint32_t>((uint8_t*)c.v + i, vec, mine, vc);
+            if (lane == 0) {
+                c.m_exp[b] = (uint8_t)me;
+                c.v_exp[b] = (uint8_t)ve;
+            }
+        } else {
+            store4<float, float4>((float*)c.m + i, vec, mine, m);
+            store4<float, float4>((float*)c.v + i, vec, mine, v);
+        }
+        store4<float, float4>(c.theta + i, vec, mine, th);
+        if (c.theta_lp != nullptr) {
+            const __bf16 lp[4] = {(__bf16)th[0], (__bf16)th[1], (__bf16)th[2], (__bf16)th[3]};
+            store4<__bf16, uint2>(c.theta_lp + i, vec, mine, lp);
+        }
+        if (a.zero_grad) {
+            const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+            store4<float, float4>(c.grad + i, vec, mine, zero);
+        }
+    }
+};
+
+// The update's common scalars, worked out by every workgroup: {alpha, lr, gradient scale}.  The three powers are one call of
+// expm1 on three lanes (b^t = exp(t log b)).
+__device__ __forceinline__ void schedule(const StepArgs& a, int64_t it, double norm2, float* out) {
+    const int lane = threadIdx.x & 63;
+    double e = 0.0;
+    if (a.decay_steps > 0) {
+        e = (double)it / (double)a.decay_steps;
+        if (a.staircase) e = floor(e);
+    }
+    const double t = (double)(it + 1);
+    const double power = expm1(lane == 0 ? t * a.log_beta1 : lane == 1 ? t * a.log_beta2 : e * a.log_rate);
+    const double p1 = __shfl(power, 0, 64), p2 = __shfl(power, 1, 64), rate = __shfl(power, 2, 64) + 1.0;
+    if (lane != 0) return;
+    const double lr = a.lr0 * rate;
+    out[0] = (float)(lr * sqrt(-p2) / -p1);
+    out[1] = (float)lr;
+    out[2] = a.grad_scale;
+    if (a.n_norm_parts > 0) {
+        const double norm = fabs((double)a.grad_scale) * sqrt(norm2);
+        // a norm that is not finite leaves nothing finite, as the clip of Keras
+        const float clip = norm > a.clip ? (float)((double)a.clip / norm) : 1.f;
+        out[2] = norm - norm == 0.0 ? a.grad_scale * clip : __uint_as_float(0x7fc00000u);
+    }
+}
+
+// A wave takes blocks of 256 elements, four a lane.  The first block is asked for before the scalars are worked out.
 template <int BITS>
 __global__ __launch_bounds__(256) void adamw_k(StepArgs a) {
-    __shared__ float s_alpha, s_lr, s_scale;
+    __shared__ float s[3];
     __shared__ double red[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t it = a.state[0];
+    Held<BITS> h;
+    int64_t k = blockIdx.x;
+    Chunk c{};
+    if (k < a.n_chunks) {
+        c = a.chunks[k];
+        if (wave * kBlock < c.n) h.load(c, wave, lane);
+    }
     double norm2 = 0.0;
     if (a.n_norm_parts > 0) {
         for (int i = threadIdx.x; i < a.n_norm_parts; i += 256) norm2 += a.norm_parts[i];
         for (int o = 32; o > 0; o >>= 1) norm2 += __shfl_xor(norm2, o, 64);
         if (lane == 0) red[wave] = norm2;
         __syncthreads();
+        norm2 = red[0] + red[1] + red[2] + red[3];
     }
-    if (threadIdx.x == 0) {
-        double lr = a.lr0;
-        if (a.decay_steps > 0) {
-            double e = (double)it / (double)a.decay_steps;
-            if (a.staircase) e = floor(e);
-            lr *= exp(e * a.log_rate);
-        }
-        const double t = (double)(it + 1);
-        s_alpha = (float)(lr * sqrt(-expm1(t * a.log_beta2)) / -expm1(t * a.log_beta1));
-        s_lr = (float)lr;
-        float scale = a.grad_scale;
-        if (a.n_norm_parts > 0) {
-            const double norm = fabs((double)a.grad_scale) * sqrt(red[0] + red[1] + red[2] + red[3]);
-            // a norm that is not finite leaves nothing finite, as the clip of Keras
-            const float clip = norm > a.clip ? (float)((double)a.clip / norm) : 1.f;
-            scale = norm - norm == 0.0 ? a.grad_scale * clip : __uint_as_float(0x7fc00000u);
-        }
-        s_scale = scale;
-    }
+    if (wave == 0) schedule(a, it, norm2, s);
     __syncthreads();
-    const float alpha = s_alpha, lr = s_lr, scale = s_scale;
+    const float alpha = s[0], lr = s[1], scale = s[2];
     const uint64_t key = mix64(mix64((uint64_t)it) ^ a.seed);
-    for (int64_t k = blockIdx.x; k < a.n_chunks; k += gridDim.x) {
-        const Chunk ck = a.chunks[k];
-        const Tensor t = a.tensors[ck.tensor];
-        const float lr_decay = lr * t.decay;
-        for (int b = wave; b < kChunk / kBlock; b += 4) {
-            const int64_t i0 = (int64_t)ck.index * kChunk + b * kBlock;
-            if (i0 >= t.n) break;
-            const int64_t i = i0 + 4 * lane;
-            const int mine = t.n - i >= 4 ? 4 : t.n - i > 0 ? (int)(t.n - i) : 0;
-            float th[4], g[4], m[4], v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                th[e] = e < mine ? t.theta[i + e] : 0.f;
-                g[e] = e < mine ? t.grad[i + e] : 0.f;
-            }
-            const int64_t block = i0 / kBlock;
-            if (BITS == 8) {
-                const int me = t.m_exp[block], ve = t.v_exp[block];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    m[e] = e < mine ? first_value(((const uint8_t*)t.m)[i + e], me) : 0.f;
-                    v[e] = e < mine ? second_value(((const uint8_t*)t.v)[i + e], ve) : 0.f;
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    m[e] = e < mine ? ((const float*)t.m)[i + e] : 0.f;
-                    v[e] = e < mine ? ((const float*)t.v)[i + e] : 0.f;
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (e < mine) update(th[e], m[e], v[e], g[e], a, scale, alpha, lr_decay);
-            if (BITS == 8) {
-                uint32_t ml = 0, vl = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t mb = __float_as_uint(m[e]) & 0x7fffffffu, vb = __float_as_uint(v[e]) & 0x7fffffffu;
-                    ml = mb > ml ? mb : ml;
-                    vl = vb > vl ? vb : vl;
-                }
-                const int me = block_exponent(wave_max(ml)), ve = block_exponent(wave_max(vl));
-                const uint64_t pair = (uint64_t)((t.first_block + block) * (kBlock / 2) + 2 * lane);
-                const uint64_t h0 = mix64(pair ^ key), h1 = mix64((pair + 1) ^ key);
-                const uint32_t r[4] = {(uint32_t)h0, (uint32_t)(h0 >> 32), (uint32_t)h1, (uint32_t)(h1 >> 32)};
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (e < mine) {
-                        ((uint8_t*)t.m)[i + e] = (uint8_t)first_code(m[e], me, r[e] & 0xffffu);
-                        ((uint8_t*)t.v)[i + e] = (uint8_t)second_code(v[e], ve, r[e] >> 16);
-                    }
-                if (lane == 0) {
-                    t.m_exp[block] = (uint8_t)me;
-                    t.v_exp[block] = (uint8_t)ve;
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (e < mine) {
-                        ((float*)t.m)[i + e] = m[e];
-                        ((float*)t.v)[i + e] = v[e];
-                    }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (e < mine) {
-                    t.theta[i + e] = th[e];
-                    if (t.theta_lp != nullptr) t.theta_lp[i + e] = (__bf16)th[e];
-                    if (a.zero_grad) t.grad[i + e] = 0.f;
-                }
+    while (k < a.n_chunks) {
+        const float lr_decay = lr * c.decay;
+        for (int b = wave; b * kBlock < c.n; b += 4) {
+            if (b != wave || k != blockIdx.x) h.load(c, b, lane);
+            h.step(c, b, lane, a, scale, alpha, lr_decay, key);
         }
+        k += gridDim.x;
+        if (k < a.n_chunks) c = a.chunks[k];
     }
     // the workgroup that arrives last advances the count: every workgroup has read it by then
     __syncthreads();
@@ -246,10 +302,22 @@ __global__ __launch_bounds__(256) void adamw_k(StepArgs a) {
     }
 }
 
+// Four codes a thread where codes and output allow it (VEC), n4 groups of four; then the last n % 4 one by one.
 template <bool SECOND>
 __global__ __launch_bounds__(256) void adamw_decode_k(const uint8_t* __restrict__ code, const uint8_t* __restrict__ exps,
-                                                       float* __restrict__ out, int64_t n) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+                                                       float* __restrict__ out, int64_t n, int64_t n4) {
+    const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, stride = (int64_t)gridDim.x * 256;
+    for (int64_t i = first; i < n4; i += stride) {
+        const uint32_t q = reinterpret_cast<const uint32_t*>(code)[i];
+        const int e = exps[i / (kBlock / 4)];
+        float4 o;
+        o.x = SECOND ? second_value(q & 0xffu, e) : first_value(q & 0xffu, e);
+        o.y = SECOND ? second_value(q >> 8 & 0xffu, e) : first_value(q >> 8 & 0xffu, e);
+        o.z = SECOND ? second_value(q >> 16 & 0xffu, e) : first_value(q >> 16 & 0xffu, e);
+        o.w = SECOND ? second_value(q >> 24, e) : first_value(q >> 24, e);
+        reinterpret_cast<float4*>(out)[i] = o;
+    }
+    for (int64_t i = 4 * n4 + first; i < n; i += stride)
         out[i] = SECOND ? second_value(code[i], exps[i / kBlock]) : first_value(code[i], exps[i / kBlock]);
 }
 
@@ -323,7 +391,7 @@ size_t sv_adamw_plan_bytes(const sv_adamw_tensor* tensors, int n_tensors, int64_
     for (int i = 0; i < n_tensors; ++i)
         if (tensors[i].n < 0 || tensors[i].n > ((int64_t)1 << 40)) return 0;
     *n_chunks = plan_chunks(tensors, n_tensors);
-    return (size_t)n_tensors * sizeof(Tensor) + (size_t)*n_chunks * sizeof(Chunk);
+    return (size_t)*n_chunks * sizeof(Chunk);
 }
 
 int sv_adamw_plan_fill(const sv_adamw_tensor* tensors, int n_tensors, int state_bits, void* image, size_t image_bytes) {
@@ -334,17 +402,21 @@ int sv_adamw_plan_fill(const sv_adamw_tensor* tensors, int n_tensors, int state_
         const size_t need = sv_adamw_plan_bytes(tensors, n_tensors, &n_chunks);
         if (image == nullptr || image_bytes < need)
             return fail(SV_E_WORKSPACE, "sv_adamw_plan_fill: image %zu bytes < required %zu", image_bytes, need);
-        Tensor* table = (Tensor*)image;
-        Chunk* chunk = (Chunk*)(table + n_tensors);
+        Chunk* chunk = (Chunk*)image;
         int64_t block = 0;
         for (int i = 0; i < n_tensors; ++i) {
             const sv_adamw_tensor& e = tensors[i];
             const uintptr_t state_align = state_bits == 8 ? 4 : 16;
             const bool vec = (uintptr_t)e.theta % 16 == 0 && (uintptr_t)e.grad % 16 == 0 && (uintptr_t)e.m % state_align == 0 &&
                              (uintptr_t)e.v % state_align == 0 && (uintptr_t)e.theta_bf16 % 8 == 0;
-            table[i] = Tensor{e.theta, e.grad, e.m, e.v, e.m_exp, e.v_exp, (__bf16*)e.theta_bf16, e.n, block, e.weight_decay, vec};
+            for (int64_t at = 0; at < e.n; at += kChunk) {
+                const int64_t left = e.n - at, each = state_bits == 8 ? 1 : 4, b = at / kBlock;
+                *chunk++ = Chunk{e.theta + at, e.grad + at, (char*)e.m + each * at, (char*)e.v + each * at,
+                                 state_bits == 8 ? e.m_exp + b : nullptr, state_bits == 8 ? e.v_exp + b : nullptr,
+                                 e.theta_bf16 ? (__bf16*)e.theta_bf16 + at : nullptr, block + b,
+                                 (int32_t)(left < kChunk ? left : kChunk), e.weight_decay, vec, 0};
+            }
             block += ceil_div(e.n, kBlock);
-            for (int64_t k = 0; k < ceil_div(e.n, kChunk); ++k) *chunk++ = Chunk{i, (int32_t)k};
         }
         return SV_OK;
     } catch (const std::bad_alloc&) {
@@ -354,10 +426,10 @@ int sv_adamw_plan_fill(const sv_adamw_tensor* tensors, int n_tensors, int state_
 
 size_t sv_adamw_workspace_bytes(void) { return kNormParts * sizeof(double); }
 
-int sv_adamw_step(const void* plan, int n_tensors, int64_t n_chunks, int state_bits, int64_t* step_state, double lr0,
+int sv_adamw_step(const void* plan, int64_t n_chunks, int state_bits, int64_t* step_state, double lr0,
                   double beta1, double beta2, float eps, int decay_steps, double decay_rate, int staircase, float grad_scale,
                   float clip_norm, uint64_t seed, int zero_grad, void* workspace, size_t workspace_bytes, sv_stream_t stream) {
-    SV_REQUIRE(plan != nullptr && step_state != nullptr && n_tensors >= 1 && n_chunks >= 0, "sv_adamw_step: bad arguments");
+    SV_REQUIRE(plan != nullptr && step_state != nullptr && n_chunks >= 0, "sv_adamw_step: bad arguments");
     SV_REQUIRE((uintptr_t)plan % 8 == 0 && (uintptr_t)step_state % 8 == 0, "sv_adamw_step: plan / state must be 8-byte aligned");
     SV_REQUIRE(state_bits == 8 || state_bits == 32, "sv_adamw_step: moments have 8 or 32 bits, not %d", state_bits);
     SV_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "sv_adamw_step: betas out of range");
@@ -367,8 +439,7 @@ int sv_adamw_step(const void* plan, int n_tensors, int64_t n_chunks, int state_b
         return fail(SV_E_WORKSPACE, "sv_adamw_step: workspace %zu bytes < required %zu", workspace_bytes, sv_adamw_workspace_bytes());
     hipStream_t st = to_stream(stream);
     StepArgs a{};
-    a.tensors = (const Tensor*)plan;
-    a.chunks = (const Chunk*)(a.tensors + n_tensors);
+    a.chunks = (const Chunk*)plan;
     a.n_chunks = n_chunks;
     a.state = step_state;
     a.lr0 = lr0;
@@ -389,7 +460,7 @@ int sv_adamw_step(const void* plan, int n_tensors, int64_t n_chunks, int state_b
     if (clip_norm > 0.f && n_chunks > 0) {
         a.norm_parts = (const double*)workspace;
         a.n_norm_parts = (int)(n_chunks < kNormParts ? n_chunks : kNormParts);
-        hipLaunchKernelGGL(grad_norm_k, dim3(a.n_norm_parts), dim3(256), 0, st, a.tensors, a.chunks, n_chunks, (double*)workspace);
+        hipLaunchKernelGGL(grad_norm_k, dim3(a.n_norm_parts), dim3(256), 0, st, a.chunks, n_chunks, (double*)workspace);
     }
     const int grid = (int)(n_chunks < 1 ? 1 : n_chunks < 2048 ? n_chunks : 2048);
     if (state_bits == 8)
@@ -403,10 +474,12 @@ int sv_adamw_decode(const uint8_t* codes, const uint8_t* exponents, float* out, 
     SV_REQUIRE(n >= 0, "sv_adamw_decode: bad arguments");
     if (n == 0) return SV_OK;
     SV_REQUIRE(codes && exponents && out, "sv_adamw_decode: bad arguments");
+    const int64_t n4 = (uintptr_t)codes % 4 == 0 && (uintptr_t)out % 16 == 0 ? n / 4 : 0;
+    const dim3 grid((unsigned)ew_grid(n4 > 0 ? n4 : n, 256, 8192));
     if (second)
-        hipLaunchKernelGGL(adamw_decode_k<true>, dim3(ew_grid(n, 256, 8192)), dim3(256), 0, to_stream(stream), codes, exponents, out, n);
+        hipLaunchKernelGGL(adamw_decode_k<true>, grid, dim3(256), 0, to_stream(stream), codes, exponents, out, n, n4);
     else
-        hipLaunchKernelGGL(adamw_decode_k<false>, dim3(ew_grid(n, 256, 8192)), dim3(256), 0, to_stream(stream), codes, exponents, out, n);
+        hipLaunchKernelGGL(adamw_decode_k<false>, grid, dim3(256), 0, to_stream(stream), codes, exponents, out, n, n4);
     return check_launch("sv_adamw_decode");
 }
 

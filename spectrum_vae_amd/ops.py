@@ -815,7 +815,7 @@ def adamw_step(plan: AdamWPlan, state, lr0, beta1, beta2, eps, decay_steps=0, de
     if state.numel() < 3:
         raise ValueError("adamw: the step state is int64[3]")
     with _on(plan._image, state) as stream:
-        check(lib.sv_adamw_step(plan._image.data_ptr(), plan.n_tensors, plan.n_chunks, plan.state_bits,
+        check(lib.sv_adamw_step(plan._image.data_ptr(), plan.n_chunks, plan.state_bits,
                                 _ptr(state, torch.int64), lr0, beta1, beta2, eps, int(decay_steps or 0), decay_rate,
                                 int(staircase), grad_scale, clip_norm, seed, int(zero_grad), plan._ws.data_ptr(),
                                 plan._ws.numel(), stream), "sv_adamw_step")

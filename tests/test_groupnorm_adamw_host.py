@@ -233,11 +233,11 @@ def test_adamw_step_refusals():
     from spectrum_vae_amd import _lib, ops
     lib = _lib.lib
 
-    def step(plan=4096, tensors=1, chunks=1, bits=32, state=4096, b1=0.9, b2=0.999, eps=1e-7, rate=0.9, clip=0.0, ws=4096,
+    def step(plan=4096, chunks=1, bits=32, state=4096, b1=0.9, b2=0.999, eps=1e-7, rate=0.9, clip=0.0, ws=4096,
              nbytes=1 << 20):
-        return lib.sv_adamw_step(plan, tensors, chunks, bits, state, 1e-3, b1, b2, eps, 10, rate, 1, 1.0, clip, 0, 0, ws, nbytes, None)
+        return lib.sv_adamw_step(plan, chunks, bits, state, 1e-3, b1, b2, eps, 10, rate, 1, 1.0, clip, 0, 0, ws, nbytes, None)
 
-    for kw in (dict(plan=None), dict(state=None), dict(tensors=0), dict(chunks=-1), dict(bits=4), dict(b1=1.0), dict(b2=-0.1),
+    for kw in (dict(plan=None), dict(state=None), dict(chunks=-1), dict(bits=4), dict(b1=1.0), dict(b2=-0.1),
                dict(eps=0.0), dict(rate=0.0), dict(clip=-1.0), dict(clip=1.0, ws=None), dict(plan=4097)):
         assert step(**kw) == -1, kw
     assert step(clip=1.0, nbytes=8) == -4
