@@ -24,7 +24,7 @@ namespace {
 
 constexpr int kBlock = 256;        // elements of an 8-bit block
 constexpr int kChunk = 4096;       // elements of one tensor that a workgroup updates at a time
-constexpr int kNormParts = 1024;   // most workgroups (partial sums) of the norm launch
+constexpr int kNormParts = 2048;   // most workgroups (partial sums) of the norm launch: eight a CU
 
 // One entry of the plan on the device: up to kChunk consecutive elements of one tensor.  Pointers are to the chunk's own first
 // element, so a workgroup gets to its data through a single dependent load.
@@ -102,15 +102,21 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
     return v;
 }
 
-// Partial sums of squares of the gradients, one a workgroup: 16 squares a thread in f32, everything else in f64.
+// Partial sums of squares of the gradients, one a workgroup: 16 squares a thread in f32, everything else in f64.  A workgroup's
+// next entry is asked for ahead of the current one's data.
 __global__ __launch_bounds__(256) void grad_norm_k(const Chunk* __restrict__ chunks, int64_t n_chunks, double* __restrict__ parts) {
     __shared__ double red[4];
     double sum = 0.0;
-    for (int64_t k = blockIdx.x; k < n_chunks; k += gridDim.x) {
-        const float* g = chunks[k].grad;
-        const int n = chunks[k].n;
+    int64_t k = blockIdx.x;
+    const float* g = k < n_chunks ? chunks[k].grad : nullptr;
+    int n = k < n_chunks ? chunks[k].n : 0, vec = k < n_chunks ? chunks[k].vec : 0;
+    while (k < n_chunks) {
+        k += gridDim.x;
+        const Chunk* next = chunks + (k < n_chunks ? k : 0);
+        const float* g_next = next->grad;
+        const int n_next = next->n, vec_next = next->vec;
         float s = 0.f;
-        if (chunks[k].vec && n == kChunk) {
+        if (vec && n == kChunk) {
             float4 q[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) q[u] = reinterpret_cast<const float4*>(g)[threadIdx.x + 256 * u];
@@ -120,6 +126,9 @@ __global__ __launch_bounds__(256) void grad_norm_k(const Chunk* __restrict__ chu
             for (int i = threadIdx.x; i < n; i += 256) s = fmaf(g[i], g[i], s);
         }
         sum += (double)s;
+        g = g_next;
+        n = n_next;
+        vec = vec_next;
     }
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
@@ -128,22 +137,24 @@ __global__ __launch_bounds__(256) void grad_norm_k(const Chunk* __restrict__ chu
 }
 
 // Four consecutive elements of a lane: VEC as one access, else the first `mine` one by one (the others read as 0).
-template <typename E, typename Q>
+// FAR: around the caches (nontemporal), for data that will not be there any more when it is used again.
+template <bool FAR, typename E, typename Q>
 __device__ __forceinline__ void load4(const E* p, bool vec, int mine, E (&out)[4]) {
     if (vec) {
-        const Q q = *reinterpret_cast<const Q*>(p);
+        const Q q = FAR ? __builtin_nontemporal_load(reinterpret_cast<const Q*>(p)) : *reinterpret_cast<const Q*>(p);
         __builtin_memcpy(out, &q, sizeof(q));
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) out[e] = e < mine ? p[e] : (E)0;
     }
 }
-template <typename E, typename Q>
+template <bool FAR, typename E, typename Q>
 __device__ __forceinline__ void store4(E* p, bool vec, int mine, const E (&in)[4]) {
     if (vec) {
         Q q;
         __builtin_memcpy(&q, in, sizeof(q));
-        *reinterpret_cast<Q*>(p) = q;
+        if (FAR) __builtin_nontemporal_store(q, reinterpret_cast<Q*>(p));
+        else *reinterpret_cast<Q*>(p) = q;
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -151,8 +162,11 @@ __device__ __forceinline__ void store4(E* p, bool vec, int mine, const E (&in)[4
     }
 }
 
+typedef float Float4 __attribute__((ext_vector_type(4)));
+typedef uint32_t Word2 __attribute__((ext_vector_type(2)));
+
 // What a lane holds of a block of 256 elements.
-template <int BITS>
+template <int BITS, bool FAR>
 struct Held {
     float th[4], g[4], m[4], v[4];
     uint8_t mc[4], vc[4];
@@ -163,16 +177,16 @@ struct Held {
         const int i = b * kBlock + 4 * lane;
         mine = c.n - i >= 4 ? 4 : c.n - i > 0 ? c.n - i : 0;
         vec = c.vec && c.n - b * kBlock >= kBlock;  // the same for the whole wave
-        load4<float, float4>(c.theta + i, vec, mine, th);
-        load4<float, float4>(c.grad + i, vec, mine, g);
+        load4<FAR, float, Float4>(c.theta + i, vec, mine, th);
+        load4<FAR, float, Float4>(c.grad + i, vec, mine, g);
         if (BITS == 8) {
             me = c.m_exp[b];
             ve = c.v_exp[b];
-            load4<uint8_t, uint32_t>((const uint8_t*)c.m + i, vec, mine, mc);
-            load4<uint8_t, uint32_t>((const uint8_t*)c.v + i, vec, mine, vc);
+            load4<FAR, uint8_t, uint32_t>((const uint8_t*)c.m + i, vec, mine, mc);
+            load4<FAR, uint8_t, uint32_t>((const uint8_t*)c.v + i, vec, mine, vc);
         } else {
-            load4<float, float4>((const float*)c.m + i, vec, mine, m);
-            load4<float, float4>((const float*)c.v + i, vec, mine, v);
+            load4<FAR, float, Float4>((const float*)c.m + i, vec, mine, m);
+            load4<FAR, float, Float4>((const float*)c.v + i, vec, mine, v);
         }
     }
 
@@ -206,24 +220,24 @@ struct Held {
                 mc[e] = (uint8_t)first_code(m[e], me, r[e] & 0xffffu);
                 vc[e] = (uint8_t)second_code(v[e], ve, r[e] >> 16);
             }
-            store4<uint8_t, uint32_t>((uint8_t*)c.m + i, vec, mine, mc);
-            store4<uint8_t, uint32_t>((uint8_t*)c.v + i, vec, mine, vc);
+            store4<FAR, uint8_t, uint32_t>((uint8_t*)c.m + i, vec, mine, mc);
+            store4<FAR, uint8_t, uint32_t>((uint8_t*)c.v + i, vec, mine, vc);
             if (lane == 0) {
                 c.m_exp[b] = (uint8_t)me;
                 c.v_exp[b] = (uint8_t)ve;
             }
         } else {
-            store4<float, float4>((float*)c.m + i, vec, mine, m);
-            store4<float, float4>((float*)c.v + i, vec, mine, v);
+            store4<FAR, float, Float4>((float*)c.m + i, vec, mine, m);
+            store4<FAR, float, Float4>((float*)c.v + i, vec, mine, v);
         }
-        store4<float, float4>(c.theta + i, vec, mine, th);
+        store4<FAR, float, Float4>(c.theta + i, vec, mine, th);
         if (c.theta_lp != nullptr) {
             const __bf16 lp[4] = {(__bf16)th[0], (__bf16)th[1], (__bf16)th[2], (__bf16)th[3]};
-            store4<__bf16, uint2>(c.theta_lp + i, vec, mine, lp);
+            store4<FAR, __bf16, Word2>(c.theta_lp + i, vec, mine, lp);
         }
         if (a.zero_grad) {
             const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-            store4<float, float4>(c.grad + i, vec, mine, zero);
+            store4<FAR, float, Float4>(c.grad + i, vec, mine, zero);
         }
     }
 };
@@ -254,13 +268,13 @@ __device__ __forceinline__ void schedule(const StepArgs& a, int64_t it, double n
 }
 
 // A wave takes blocks of 256 elements, four a lane.  The first block is asked for before the scalars are worked out.
-template <int BITS>
+template <int BITS, bool FAR>
 __global__ __launch_bounds__(256) void adamw_k(StepArgs a) {
     __shared__ float s[3];
     __shared__ double red[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t it = a.state[0];
-    Held<BITS> h;
+    Held<BITS, FAR> h;
     int64_t k = blockIdx.x;
     Chunk c{};
     if (k < a.n_chunks) {
@@ -463,10 +477,11 @@ int sv_adamw_step(const void* plan, int64_t n_chunks, int state_bits, int64_t* s
         hipLaunchKernelGGL(grad_norm_k, dim3(a.n_norm_parts), dim3(256), 0, st, a.chunks, n_chunks, (double*)workspace);
     }
     const int grid = (int)(n_chunks < 1 ? 1 : n_chunks < 2048 ? n_chunks : 2048);
-    if (state_bits == 8)
-        hipLaunchKernelGGL(adamw_k<8>, dim3(grid), dim3(256), 0, st, a);
-    else
-        hipLaunchKernelGGL(adamw_k<32>, dim3(grid), dim3(256), 0, st, a);
+    // more than the caches between the chip and the memory hold (256 MB): nothing of it is found there at the next step
+    // (101 M weights: 555 against 515 us with 32-bit moments, 352 against 338 with 8-bit ones)
+    const bool far = n_chunks * kChunk * (state_bits == 8 ? 10 : 16) > ((int64_t)256 << 20);
+    const auto kernel = state_bits == 8 ? (far ? adamw_k<8, true> : adamw_k<8, false>) : (far ? adamw_k<32, true> : adamw_k<32, false>);
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, st, a);
     return check_launch("sv_adamw_step");
 }
 

@@ -533,23 +533,33 @@ class _on:
     """``with _on(x, ...) as stream``: the device all these tensors are on becomes the current one for the block; ``stream``
     is its current stream."""
 
+    __slots__ = ("device", "guard")
+
     def __init__(self, first, *rest):
-        dev = first.device
+        dev = first.get_device()
         for t in rest:
-            if t is not None and t.device != dev:
-                raise ValueError(f"tensors on {dev} and {t.device}: a launch takes tensors of one device")
-        if not first.is_cuda:
-            raise _lib.SpectrumHipError(f"tensor is on {dev}: the HIP path needs device tensors (no CPU fallback)")
-        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+            if t is not None and t.get_device() != dev:
+                raise ValueError(f"tensors on {first.device} and {t.device}: a launch takes tensors of one device")
+        if dev < 0:
+            raise _lib.SpectrumHipError(f"tensor is on {first.device}: the HIP path needs device tensors (no CPU fallback)")
+        self.device = dev
+        self.guard = None if dev == torch.cuda.current_device() else torch.cuda.device(dev)
 
     def __enter__(self):
         if self.guard is not None:
             self.guard.__enter__()
-        return _stream()
+        return torch._C._cuda_getCurrentRawStream(self.device)  # torch.cuda.current_stream() without the object around it
 
     def __exit__(self, *exc):
         if self.guard is not None:
             self.guard.__exit__(*exc)
+
+
+def _f32(t) -> Optional[int]:
+    """``_ptr`` of a float32 tensor whose device ``_on`` has seen."""
+    if t is None:
+        return None
+    return t.data_ptr() if t.dtype is torch.float32 and t.is_contiguous() else _ptr(t)
 
 
 def groupnorm_workspace(n: int, s: int, c: int, groups: int) -> int:
@@ -581,7 +591,7 @@ def groupnorm_act_fwd(x, gamma, beta, y, save_mean, save_rstd, groups: int, eps:
     bfloat16, everything else float32.  save_mean / save_rstd [N, groups]: for the backward call; both may be None."""
     n, s, c = _groupnorm_extents(x, y, gamma, beta, save_mean, save_rstd, groups)
     with _on(x, gamma, beta, y, save_mean, save_rstd, ws) as stream:
-        check(lib.sv_groupnorm_act_fwd(_aptr(x), _ptr(gamma), _ptr(beta), _aptr(y, x, "y"), _ptr(save_mean), _ptr(save_rstd),
+        check(lib.sv_groupnorm_act_fwd(_aptr(x), _f32(gamma), _f32(beta), _aptr(y, x, "y"), _f32(save_mean), _f32(save_rstd),
                                        n, s, c, groups, eps, ACT[act], alpha, *_ws_args(ws), _dt(x), stream),
               "sv_groupnorm_act_fwd")
 
@@ -595,8 +605,8 @@ def groupnorm_act_bwd(x, dy, gamma, beta, save_mean, save_rstd, dx, dgamma, dbet
     if dgamma.numel() != c or dbeta.numel() != c:
         raise ValueError(f"groupnorm: dgamma / dbeta must have the {c} channels' size")
     with _on(x, dy, gamma, beta, save_mean, save_rstd, dx, dgamma, dbeta, ws) as stream:
-        check(lib.sv_groupnorm_act_bwd(_aptr(x), _aptr(dy, x, "dy"), _ptr(gamma), _ptr(beta), _ptr(save_mean), _ptr(save_rstd),
-                                       _aptr(dx, x, "dx"), _ptr(dgamma), _ptr(dbeta), int(accumulate), n, s, c, groups,
+        check(lib.sv_groupnorm_act_bwd(_aptr(x), _aptr(dy, x, "dy"), _f32(gamma), _f32(beta), _f32(save_mean), _f32(save_rstd),
+                                       _aptr(dx, x, "dx"), _f32(dgamma), _f32(dbeta), int(accumulate), n, s, c, groups,
                                        ACT[act], alpha, *_ws_args(ws), _dt(x), stream), "sv_groupnorm_act_bwd")
 
 
