@@ -540,9 +540,10 @@ int sv_adam_keras_apply(float* theta, float* grad, float* m, float* v, int64_t n
  *      magnitude once its mantissa is rounded up to 3 bits.  A value goes to the code above it if 16 random bits say so
  *      (with the probability of its distance to the code below), a positive second moment to code 1 at least.  The bits of an
  *      element are a hash of (seed, count, the element's position: 256 * the blocks of the tensors before it + its index).
- *  A plan is a device copy of the host image that sv_adamw_plan_fill writes (sv_adamw_plan_bytes gives its size and
- *      *n_chunks, both for sv_adamw_step); it holds the tensors' addresses.  No two buffers of a plan may overlap.
- *  step_state: the 24 bytes of sv_adam_keras_step.  zero_grad: the gradients are cleared once read.
+ *  A plan is a device copy, 128-byte aligned, of the host image that sv_adamw_plan_fill writes (sv_adamw_plan_bytes gives its
+ *      size and *n_chunks); it holds the tensors' addresses and the arrival counters of the launch, so launches with one plan must
+ *      not overlap in time.  No two buffers of a plan may overlap.
+ *  step_state: 16 bytes, the count and {alpha, lr} of the last update as in sv_adam_keras_step.  zero_grad: the gradients are cleared once read.
  *  workspace: sv_adamw_workspace_bytes, 8-byte aligned; only read with clip_norm > 0.
  *  sv_adamw_decode: out[i] = the value of codes[i] (second: of a second moment) for one tensor, or for several that lie back to
  *      back in codes and exponents, each starting on a multiple of 256. */
@@ -561,7 +562,7 @@ typedef struct sv_adamw_tensor {
 size_t sv_adamw_plan_bytes(const sv_adamw_tensor* tensors, int n_tensors, int64_t* n_chunks);
 int sv_adamw_plan_fill(const sv_adamw_tensor* tensors, int n_tensors, int state_bits, void* image, size_t image_bytes);
 size_t sv_adamw_workspace_bytes(void);
-int sv_adamw_step(const void* plan, int64_t n_chunks, int state_bits, int64_t* step_state, double lr0, double beta1, double beta2,
+int sv_adamw_step(void* plan, int64_t n_chunks, int state_bits, int64_t* step_state, double lr0, double beta1, double beta2,
                   float eps, int decay_steps, double decay_rate, int staircase, float grad_scale, float clip_norm, uint64_t seed,
                   int zero_grad, void* workspace, size_t workspace_bytes, sv_stream_t stream);
 int sv_adamw_decode(const uint8_t* codes, const uint8_t* exponents, float* out, int64_t n, int second, sv_stream_t stream);

@@ -26,6 +26,9 @@ constexpr int kBlock = 256;        // elements of an 8-bit block
 constexpr int kChunk = 4096;       // elements of one tensor that a workgroup updates at a time
 constexpr int kNormParts = 2048;   // most workgroups (partial sums) of the norm launch: eight a CU
 
+// A pointer read from memory is not known to point there: without this its accesses would be flat ones, which also go by LDS.
+#define SV_GLOBAL __attribute__((address_space(1)))
+
 // One entry of the plan on the device: up to kChunk consecutive elements of one tensor.  Pointers are to the chunk's own first
 // element, so a workgroup gets to its data through a single dependent load.
 struct Chunk {
@@ -43,14 +46,21 @@ struct Chunk {
     int32_t pad;
 };
 
+constexpr unsigned kTickets = 32;
+struct alignas(128) Ticket {
+    unsigned count;
+};
+// device image: Ticket[kTickets + 1] (zero between launches), Chunk[n_chunks]
+
 struct StepArgs {
+    Ticket* tickets;
     const Chunk* chunks;
     int64_t n_chunks;
     int64_t* state;
     const double* norm_parts;
     double lr0, log_beta1, log_beta2, log_rate;
     float beta1, beta2, one_minus_beta1, one_minus_beta2, eps, grad_scale, clip;
-    int decay_steps, staircase, zero_grad, n_norm_parts;
+    int decay_steps, staircase, zero_grad, n_norm_parts, log_split;
     uint64_t seed;
 };
 
@@ -93,14 +103,26 @@ __device__ __forceinline__ void update(float& th, float& m, float& v, float g, c
     th = th - (alpha * m) * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v) + a.eps);
 }
 
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint32_t w = __shfl_xor(v, o, 64);
-        v = w > v ? w : v;
-    }
-    return v;
+// Maximum over a wave in every lane, one vector instruction a step (no LDS): within a row of 16 lanes by data-parallel
+// primitives, between rows by lane swaps.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+    const uint32_t w = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+    return w > v ? w : v;
 }
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    v = dpp_max<0xB1>(v);   // lane ^ 1
+    v = dpp_max<0x4E>(v);   // lane ^ 2
+    v = dpp_max<0x141>(v);  // the other half of 8
+    v = dpp_max<0x140>(v);  // the other half of 16
+    auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = r[0] > r[1] ? r[0] : r[1];
+    r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return r[0] > r[1] ? r[0] : r[1];
+}
+
+typedef float Float4 __attribute__((ext_vector_type(4)));
+typedef uint32_t Word2 __attribute__((ext_vector_type(2)));
 
 // Partial sums of squares of the gradients, one a workgroup: 16 squares a thread in f32, everything else in f64.  A workgroup's
 // next entry is asked for ahead of the current one's data.
@@ -117,13 +139,13 @@ __global__ __launch_bounds__(256) void grad_norm_k(const Chunk* __restrict__ chu
         const int n_next = next->n, vec_next = next->vec;
         float s = 0.f;
         if (vec && n == kChunk) {
-            float4 q[4];
+            Float4 q[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) q[u] = reinterpret_cast<const float4*>(g)[threadIdx.x + 256 * u];
+            for (int u = 0; u < 4; ++u) q[u] = ((const SV_GLOBAL Float4*)g)[threadIdx.x + 256 * u];
 #pragma unroll
             for (int u = 0; u < 4; ++u) s = fmaf(q[u].x, q[u].x, fmaf(q[u].y, q[u].y, fmaf(q[u].z, q[u].z, fmaf(q[u].w, q[u].w, s))));
         } else {
-            for (int i = threadIdx.x; i < n; i += 256) s = fmaf(g[i], g[i], s);
+            for (int i = threadIdx.x; i < n; i += 256) s = fmaf(((const SV_GLOBAL float*)g)[i], ((const SV_GLOBAL float*)g)[i], s);
         }
         sum += (double)s;
         g = g_next;
@@ -139,9 +161,10 @@ __global__ __launch_bounds__(256) void grad_norm_k(const Chunk* __restrict__ chu
 // Four consecutive elements of a lane: VEC as one access, else the first `mine` one by one (the others read as 0).
 // FAR: around the caches (nontemporal), for data that will not be there any more when it is used again.
 template <bool FAR, typename E, typename Q>
-__device__ __forceinline__ void load4(const E* p, bool vec, int mine, E (&out)[4]) {
+__device__ __forceinline__ void load4(const E* generic, bool vec, int mine, E (&out)[4]) {
+    const SV_GLOBAL E* p = (const SV_GLOBAL E*)generic;
     if (vec) {
-        const Q q = FAR ? __builtin_nontemporal_load(reinterpret_cast<const Q*>(p)) : *reinterpret_cast<const Q*>(p);
+        const Q q = FAR ? __builtin_nontemporal_load((const SV_GLOBAL Q*)p) : *(const SV_GLOBAL Q*)p;
         __builtin_memcpy(out, &q, sizeof(q));
     } else {
 #pragma unroll
@@ -149,12 +172,13 @@ __device__ __forceinline__ void load4(const E* p, bool vec, int mine, E (&out)[4
     }
 }
 template <bool FAR, typename E, typename Q>
-__device__ __forceinline__ void store4(E* p, bool vec, int mine, const E (&in)[4]) {
+__device__ __forceinline__ void store4(E* generic, bool vec, int mine, const E (&in)[4]) {
+    SV_GLOBAL E* p = (SV_GLOBAL E*)generic;
     if (vec) {
         Q q;
         __builtin_memcpy(&q, in, sizeof(q));
-        if (FAR) __builtin_nontemporal_store(q, reinterpret_cast<Q*>(p));
-        else *reinterpret_cast<Q*>(p) = q;
+        if (FAR) __builtin_nontemporal_store(q, (SV_GLOBAL Q*)p);
+        else *(SV_GLOBAL Q*)p = q;
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -162,28 +186,45 @@ __device__ __forceinline__ void store4(E* p, bool vec, int mine, const E (&in)[4
     }
 }
 
-typedef float Float4 __attribute__((ext_vector_type(4)));
-typedef uint32_t Word2 __attribute__((ext_vector_type(2)));
+template <bool FAR>
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* generic, bool vec, int mine) {
+    const SV_GLOBAL uint8_t* p = (const SV_GLOBAL uint8_t*)generic;
+    if (vec) return FAR ? __builtin_nontemporal_load((const SV_GLOBAL uint32_t*)p) : *(const SV_GLOBAL uint32_t*)p;
+    uint32_t w = 0;
+    for (int e = 0; e < mine; ++e) w |= (uint32_t)p[e] << 8 * e;
+    return w;
+}
+template <bool FAR>
+__device__ __forceinline__ void store_codes(uint8_t* generic, bool vec, int mine, uint32_t w) {
+    SV_GLOBAL uint8_t* p = (SV_GLOBAL uint8_t*)generic;
+    if (vec) {
+        if (FAR) __builtin_nontemporal_store(w, (SV_GLOBAL uint32_t*)p);
+        else *(SV_GLOBAL uint32_t*)p = w;
+    } else {
+        for (int e = 0; e < mine; ++e) p[e] = (uint8_t)(w >> 8 * e);
+    }
+}
 
 // What a lane holds of a block of 256 elements.
 template <int BITS, bool FAR>
 struct Held {
     float th[4], g[4], m[4], v[4];
-    uint8_t mc[4], vc[4];
+    uint32_t mc, vc;  // four codes each
     int me, ve, mine;
     bool vec;
 
     __device__ __forceinline__ void load(const Chunk& c, int b, int lane) {
-        const int i = b * kBlock + 4 * lane;
-        mine = c.n - i >= 4 ? 4 : c.n - i > 0 ? c.n - i : 0;
+        const uint32_t i = b * kBlock + 4 * lane;  // (unsigned: offsets then need no register pair)
+        const int left = c.n - (int)i;
+        mine = left >= 4 ? 4 : left > 0 ? left : 0;
         vec = c.vec && c.n - b * kBlock >= kBlock;  // the same for the whole wave
         load4<FAR, float, Float4>(c.theta + i, vec, mine, th);
         load4<FAR, float, Float4>(c.grad + i, vec, mine, g);
         if (BITS == 8) {
-            me = c.m_exp[b];
-            ve = c.v_exp[b];
-            load4<FAR, uint8_t, uint32_t>((const uint8_t*)c.m + i, vec, mine, mc);
-            load4<FAR, uint8_t, uint32_t>((const uint8_t*)c.v + i, vec, mine, vc);
+            me = ((const SV_GLOBAL uint8_t*)c.m_exp)[b];
+            ve = ((const SV_GLOBAL uint8_t*)c.v_exp)[b];
+            mc = load_codes<FAR>((const uint8_t*)c.m + i, vec, mine);
+            vc = load_codes<FAR>((const uint8_t*)c.v + i, vec, mine);
         } else {
             load4<FAR, float, Float4>((const float*)c.m + i, vec, mine, m);
             load4<FAR, float, Float4>((const float*)c.v + i, vec, mine, v);
@@ -192,12 +233,12 @@ struct Held {
 
     __device__ __forceinline__ void step(const Chunk& c, int b, int lane, const StepArgs& a, float scale, float alpha,
                                          float lr_decay, uint64_t key) {
-        const int i = b * kBlock + 4 * lane;
+        const uint32_t i = b * kBlock + 4 * lane;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if (BITS == 8) {
-                m[e] = first_value(mc[e], me);
-                v[e] = second_value(vc[e], ve);
+                m[e] = first_value(mc >> 8 * e & 0xffu, me);
+                v[e] = second_value(vc >> 8 * e & 0xffu, ve);
             }
             update(th[e], m[e], v[e], g[e], a, scale, alpha, lr_decay);
         }
@@ -215,16 +256,17 @@ struct Held {
             const uint64_t pair = (uint64_t)((c.block + b) * (kBlock / 2) + 2 * lane);
             const uint64_t h0 = mix64(pair ^ key), h1 = mix64((pair + 1) ^ key);
             const uint32_t r[4] = {(uint32_t)h0, (uint32_t)(h0 >> 32), (uint32_t)h1, (uint32_t)(h1 >> 32)};
+            mc = vc = 0;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                mc[e] = (uint8_t)first_code(m[e], me, r[e] & 0xffffu);
-                vc[e] = (uint8_t)second_code(v[e], ve, r[e] >> 16);
+                mc |= first_code(m[e], me, r[e] & 0xffffu) << 8 * e;
+                vc |= second_code(v[e], ve, r[e] >> 16) << 8 * e;
             }
-            store4<FAR, uint8_t, uint32_t>((uint8_t*)c.m + i, vec, mine, mc);
-            store4<FAR, uint8_t, uint32_t>((uint8_t*)c.v + i, vec, mine, vc);
+            store_codes<FAR>((uint8_t*)c.m + i, vec, mine, mc);
+            store_codes<FAR>((uint8_t*)c.v + i, vec, mine, vc);
             if (lane == 0) {
-                c.m_exp[b] = (uint8_t)me;
-                c.v_exp[b] = (uint8_t)ve;
+                ((SV_GLOBAL uint8_t*)c.m_exp)[b] = (uint8_t)me;
+                ((SV_GLOBAL uint8_t*)c.v_exp)[b] = (uint8_t)ve;
             }
         } else {
             store4<FAR, float, Float4>((float*)c.m + i, vec, mine, m);
@@ -242,8 +284,8 @@ struct Held {
     }
 };
 
-// The update's common scalars, worked out by every workgroup: {alpha, lr, gradient scale}.  The three powers are one call of
-// expm1 on three lanes (b^t = exp(t log b)).
+// The update's common scalars, worked out by every workgroup: {alpha, lr, gradient scale}.  The three powers are one
+// call of exp on three lanes (b^t = exp(t log b)).
 __device__ __forceinline__ void schedule(const StepArgs& a, int64_t it, double norm2, float* out) {
     const int lane = threadIdx.x & 63;
     double e = 0.0;
@@ -252,11 +294,11 @@ __device__ __forceinline__ void schedule(const StepArgs& a, int64_t it, double n
         if (a.staircase) e = floor(e);
     }
     const double t = (double)(it + 1);
-    const double power = expm1(lane == 0 ? t * a.log_beta1 : lane == 1 ? t * a.log_beta2 : e * a.log_rate);
-    const double p1 = __shfl(power, 0, 64), p2 = __shfl(power, 1, 64), rate = __shfl(power, 2, 64) + 1.0;
+    const double power = exp(lane == 0 ? t * a.log_beta1 : lane == 1 ? t * a.log_beta2 : e * a.log_rate);
+    const double p1 = __shfl(power, 0, 64), p2 = __shfl(power, 1, 64), rate = __shfl(power, 2, 64);
     if (lane != 0) return;
     const double lr = a.lr0 * rate;
-    out[0] = (float)(lr * sqrt(-p2) / -p1);
+    out[0] = (float)(lr * sqrt(1.0 - p2) / (1.0 - p1));  // 1 - b^t loses at most 2^-53 / (1 - b) of itself
     out[1] = (float)lr;
     out[2] = a.grad_scale;
     if (a.n_norm_parts > 0) {
@@ -267,19 +309,37 @@ __device__ __forceinline__ void schedule(const StepArgs& a, int64_t it, double n
     }
 }
 
-// A wave takes blocks of 256 elements, four a lane.  The first block is asked for before the scalars are worked out.
+// Whether this is the last workgroup of the launch to get here (one thread asks).  With more than 64 of them arrivals are counted
+// in kTickets places of a cache line each first: on a single counter, 850 workgroups queue for 8 us.  All counters are left
+// zero.
+__device__ __forceinline__ bool last_of(Ticket& t, unsigned all) {
+    if (__hip_atomic_fetch_add(&t.count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != all - 1) return false;
+    __hip_atomic_store(&t.count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return true;
+}
+__device__ __forceinline__ bool last_to_arrive(Ticket* t) {
+    if (gridDim.x <= 64) return last_of(t[kTickets], gridDim.x);
+    const unsigned at = blockIdx.x % kTickets;
+    return last_of(t[at], (gridDim.x - at + kTickets - 1) / kTickets) && last_of(t[kTickets], kTickets);
+}
+
+// A wave takes blocks of 256 elements, four a lane: every 4 * 2^log_split-th block of a chunk, 2^log_split workgroups a chunk (so
+// that few chunks spread over more CUs).  The first block is asked for before the common scalars are worked out.
+// A CU holds kResident workgroups (64 registers a thread, 80 with 8-bit moments); no launch has more of them at once.
+template <int BITS> constexpr int kResident = BITS == 8 ? 6 : 8;
 template <int BITS, bool FAR>
-__global__ __launch_bounds__(256) void adamw_k(StepArgs a) {
+__global__ __launch_bounds__(256, kResident<BITS>) void adamw_k(StepArgs a) {
     __shared__ float s[3];
     __shared__ double red[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t it = a.state[0];
+    const int64_t it = a.state[0], items = a.n_chunks << a.log_split;
     Held<BITS, FAR> h;
-    int64_t k = blockIdx.x;
+    int64_t k = blockIdx.x;  // item: chunk k >> log_split, its blocks from 4 times the rest on
+    int first = 4 * (int)(k & ((1 << a.log_split) - 1)) + wave;
     Chunk c{};
-    if (k < a.n_chunks) {
-        c = a.chunks[k];
-        if (wave * kBlock < c.n) h.load(c, wave, lane);
+    if (k < items) {
+        c = a.chunks[k >> a.log_split];
+        if (first * kBlock < c.n) h.load(c, first, lane);
     }
     double norm2 = 0.0;
     if (a.n_norm_parts > 0) {
@@ -293,43 +353,42 @@ __global__ __launch_bounds__(256) void adamw_k(StepArgs a) {
     __syncthreads();
     const float alpha = s[0], lr = s[1], scale = s[2];
     const uint64_t key = mix64(mix64((uint64_t)it) ^ a.seed);
-    while (k < a.n_chunks) {
+    while (k < items) {
         const float lr_decay = lr * c.decay;
-        for (int b = wave; b * kBlock < c.n; b += 4) {
-            if (b != wave || k != blockIdx.x) h.load(c, b, lane);
+        for (int b = first; b * kBlock < c.n; b += 4 << a.log_split) {
+            if (b != first || k != blockIdx.x) h.load(c, b, lane);
             h.step(c, b, lane, a, scale, alpha, lr_decay, key);
         }
         k += gridDim.x;
-        if (k < a.n_chunks) c = a.chunks[k];
+        if (k < items) {
+            first = 4 * (int)(k & ((1 << a.log_split) - 1)) + wave;
+            c = a.chunks[k >> a.log_split];
+        }
     }
     // the workgroup that arrives last advances the count: every workgroup has read it by then
     __syncthreads();
-    if (threadIdx.x == 0) {
-        unsigned int* ticket = reinterpret_cast<unsigned int*>(a.state + 2);
-        const unsigned int prev = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (prev == gridDim.x - 1) {
-            a.state[0] = it + 1;
-            reinterpret_cast<float*>(a.state + 1)[0] = alpha;
-            reinterpret_cast<float*>(a.state + 1)[1] = lr;
-            __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
+    if (threadIdx.x == 0 && last_to_arrive(a.tickets)) {
+        a.state[0] = it + 1;
+        reinterpret_cast<float*>(a.state + 1)[0] = alpha;
+        reinterpret_cast<float*>(a.state + 1)[1] = lr;
     }
 }
 
 // Four codes a thread where codes and output allow it (VEC), n4 groups of four; then the last n % 4 one by one.
-template <bool SECOND>
+template <bool SECOND, bool FAR>
 __global__ __launch_bounds__(256) void adamw_decode_k(const uint8_t* __restrict__ code, const uint8_t* __restrict__ exps,
                                                        float* __restrict__ out, int64_t n, int64_t n4) {
     const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, stride = (int64_t)gridDim.x * 256;
     for (int64_t i = first; i < n4; i += stride) {
         const uint32_t q = reinterpret_cast<const uint32_t*>(code)[i];
         const int e = exps[i / (kBlock / 4)];
-        float4 o;
+        Float4 o;
         o.x = SECOND ? second_value(q & 0xffu, e) : first_value(q & 0xffu, e);
         o.y = SECOND ? second_value(q >> 8 & 0xffu, e) : first_value(q >> 8 & 0xffu, e);
         o.z = SECOND ? second_value(q >> 16 & 0xffu, e) : first_value(q >> 16 & 0xffu, e);
         o.w = SECOND ? second_value(q >> 24, e) : first_value(q >> 24, e);
-        reinterpret_cast<float4*>(out)[i] = o;
+        if (FAR) __builtin_nontemporal_store(o, reinterpret_cast<Float4*>(out) + i);
+        else reinterpret_cast<Float4*>(out)[i] = o;
     }
     for (int64_t i = 4 * n4 + first; i < n; i += stride)
         out[i] = SECOND ? second_value(code[i], exps[i / kBlock]) : first_value(code[i], exps[i / kBlock]);
@@ -405,7 +464,7 @@ size_t sv_adamw_plan_bytes(const sv_adamw_tensor* tensors, int n_tensors, int64_
     for (int i = 0; i < n_tensors; ++i)
         if (tensors[i].n < 0 || tensors[i].n > ((int64_t)1 << 40)) return 0;
     *n_chunks = plan_chunks(tensors, n_tensors);
-    return (size_t)*n_chunks * sizeof(Chunk);
+    return (kTickets + 1) * sizeof(Ticket) + (size_t)*n_chunks * sizeof(Chunk);
 }
 
 int sv_adamw_plan_fill(const sv_adamw_tensor* tensors, int n_tensors, int state_bits, void* image, size_t image_bytes) {
@@ -416,7 +475,8 @@ int sv_adamw_plan_fill(const sv_adamw_tensor* tensors, int n_tensors, int state_
         const size_t need = sv_adamw_plan_bytes(tensors, n_tensors, &n_chunks);
         if (image == nullptr || image_bytes < need)
             return fail(SV_E_WORKSPACE, "sv_adamw_plan_fill: image %zu bytes < required %zu", image_bytes, need);
-        Chunk* chunk = (Chunk*)image;
+        memset(image, 0, (kTickets + 1) * sizeof(Ticket));
+        Chunk* chunk = (Chunk*)((char*)image + (kTickets + 1) * sizeof(Ticket));
         int64_t block = 0;
         for (int i = 0; i < n_tensors; ++i) {
             const sv_adamw_tensor& e = tensors[i];
@@ -440,11 +500,11 @@ int sv_adamw_plan_fill(const sv_adamw_tensor* tensors, int n_tensors, int state_
 
 size_t sv_adamw_workspace_bytes(void) { return kNormParts * sizeof(double); }
 
-int sv_adamw_step(const void* plan, int64_t n_chunks, int state_bits, int64_t* step_state, double lr0,
+int sv_adamw_step(void* plan, int64_t n_chunks, int state_bits, int64_t* step_state, double lr0,
                   double beta1, double beta2, float eps, int decay_steps, double decay_rate, int staircase, float grad_scale,
                   float clip_norm, uint64_t seed, int zero_grad, void* workspace, size_t workspace_bytes, sv_stream_t stream) {
     SV_REQUIRE(plan != nullptr && step_state != nullptr && n_chunks >= 0, "sv_adamw_step: bad arguments");
-    SV_REQUIRE((uintptr_t)plan % 8 == 0 && (uintptr_t)step_state % 8 == 0, "sv_adamw_step: plan / state must be 8-byte aligned");
+    SV_REQUIRE((uintptr_t)plan % 128 == 0 && (uintptr_t)step_state % 8 == 0, "sv_adamw_step: plan must be 128-byte, state 8-byte aligned");
     SV_REQUIRE(state_bits == 8 || state_bits == 32, "sv_adamw_step: moments have 8 or 32 bits, not %d", state_bits);
     SV_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "sv_adamw_step: betas out of range");
     SV_REQUIRE(eps > 0.f && clip_norm >= 0.f && (decay_steps <= 0 || decay_rate > 0.0), "sv_adamw_step: epsilon and the decay rate must be positive, the clip not negative");
@@ -453,7 +513,8 @@ int sv_adamw_step(const void* plan, int64_t n_chunks, int state_bits, int64_t* s
         return fail(SV_E_WORKSPACE, "sv_adamw_step: workspace %zu bytes < required %zu", workspace_bytes, sv_adamw_workspace_bytes());
     hipStream_t st = to_stream(stream);
     StepArgs a{};
-    a.chunks = (const Chunk*)plan;
+    a.tickets = (Ticket*)plan;
+    a.chunks = (const Chunk*)(a.tickets + kTickets + 1);
     a.n_chunks = n_chunks;
     a.state = step_state;
     a.lr0 = lr0;
@@ -476,7 +537,10 @@ int sv_adamw_step(const void* plan, int64_t n_chunks, int state_bits, int64_t* s
         a.n_norm_parts = (int)(n_chunks < kNormParts ? n_chunks : kNormParts);
         hipLaunchKernelGGL(grad_norm_k, dim3(a.n_norm_parts), dim3(256), 0, st, a.chunks, n_chunks, (double*)workspace);
     }
-    const int grid = (int)(n_chunks < 1 ? 1 : n_chunks < 2048 ? n_chunks : 2048);
+    const int most = 256 * (state_bits == 8 ? kResident<8> : kResident<32>);
+    a.log_split = 4 * n_chunks <= most ? 2 : 2 * n_chunks <= most ? 1 : 0;  // a block a wave where the chip holds that at once
+    const int64_t items = n_chunks << a.log_split;
+    const int grid = (int)(items < 1 ? 1 : items < most ? items : most);
     // more than the caches between the chip and the memory hold (256 MB): nothing of it is found there at the next step
     // (101 M weights: 555 against 515 us with 32-bit moments, 352 against 338 with 8-bit ones)
     const bool far = n_chunks * kChunk * (state_bits == 8 ? 10 : 16) > ((int64_t)256 << 20);
@@ -491,10 +555,10 @@ int sv_adamw_decode(const uint8_t* codes, const uint8_t* exponents, float* out, 
     SV_REQUIRE(codes && exponents && out, "sv_adamw_decode: bad arguments");
     const int64_t n4 = (uintptr_t)codes % 4 == 0 && (uintptr_t)out % 16 == 0 ? n / 4 : 0;
     const dim3 grid((unsigned)ew_grid(n4 > 0 ? n4 : n, 256, 8192));
-    if (second)
-        hipLaunchKernelGGL(adamw_decode_k<true>, grid, dim3(256), 0, to_stream(stream), codes, exponents, out, n, n4);
-    else
-        hipLaunchKernelGGL(adamw_decode_k<false>, grid, dim3(256), 0, to_stream(stream), codes, exponents, out, n, n4);
+    const bool far = n * 4 > ((int64_t)256 << 20);
+    const auto kernel = second ? (far ? adamw_decode_k<true, true> : adamw_decode_k<true, false>)
+                               : (far ? adamw_decode_k<false, true> : adamw_decode_k<false, false>);
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, to_stream(stream), codes, exponents, out, n, n4);
     return check_launch("sv_adamw_decode");
 }
 

@@ -490,12 +490,13 @@ __global__ __launch_bounds__(NT) void gn_bwd_held_k(GnArgs a) {
 // ------------------------------------------------------------------------------------------------ streamed
 // Workgroup -> (sample, chunk of rows, slab of channels); 256 threads, P = CB / V <= 256 pieces a row, rows r, r + 256 / P, ...
 constexpr int kStreamThreads = 256;
+__host__ __device__ __forceinline__ bool lanes_share(int P) { return P <= 64 && (P & (P - 1)) == 0; }
 // Per chunk and channel.  Forward: mean and sum of squared deviations (about the chunk's first row, then moved to the mean).
 // Backward: sum dz, sum dz xhat.
 // Eight workgroups a CU: 2048 of them are resident at once (with eight bf16 channels a thread, backward, half of them).
 template <typename T, int V, bool BWD>
 __global__ __launch_bounds__(kStreamThreads, BWD && V == 8 ? 4 : 8) void gn_sums_k(GnArgs a) {
-    extern __shared__ float sm[];  // [rows at a time][channels of a slab], one quantity at a time | [channels] of the first one
+    extern __shared__ float sm[];  // [2][rows at a time, or waves][channels of a slab] | [channels] of the first row
     constexpr int NT = kStreamThreads, U = BWD ? 2 : V == 8 ? 4 : 8;  // pieces of each tensor in flight
     const int slab = (int)(blockIdx.x % a.slabs);
     const int64_t i = blockIdx.x / a.slabs, n = i / a.chunks, chunk = i % a.chunks;
@@ -522,11 +523,9 @@ __global__ __launch_bounds__(kStreamThreads, BWD && V == 8 ? 4 : 8) void gn_sums
                 ga[e] = a.gamma[c0 + e];
                 be[e] = a.beta[c0 + e];
             }
-        } else {
-            const Piece<T, V> first = piece_at<Q_>(x, col);
-#pragma unroll
-            for (int e = 0; e < V; ++e) mu[e] = get<T, V>(first, e);
         }
+        Piece<T, V> pivot;
+        if (!BWD) pivot = piece_at<Q_>(x, col);
         const auto row = [&](const Piece<T, V>& bx, const Piece<T, V>& bg, auto act) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
@@ -542,6 +541,12 @@ __global__ __launch_bounds__(kStreamThreads, BWD && V == 8 ? 4 : 8) void gn_sums
                 }
             }
         };
+        const auto about = [&] {  // behind the first loads, not ahead of them: the first row is waited for with them
+            if (BWD) return;
+            forget(pivot);
+#pragma unroll
+            for (int e = 0; e < V; ++e) mu[e] = get<T, V>(pivot, e);
+        };
         const auto all = [&](auto act) {
             int at = r;
             for (; at + (U - 1) * rpb < rows; at += U * rpb) {
@@ -551,9 +556,11 @@ __global__ __launch_bounds__(kStreamThreads, BWD && V == 8 ? 4 : 8) void gn_sums
                     bx[u] = piece_at<Q_>(x, col + (at + u * rpb) * pitch);
                     if (BWD) bg[u] = piece_at<Q_>(dy, col + (at + u * rpb) * pitch);
                 }
+                about();
 #pragma unroll
                 for (int u = 0; u < U; ++u) row(bx[u], bg[u], act);
             }
+            about();
             for (; at < rows; at += rpb) {
                 const Piece<T, V> bx = piece_at<Q_>(x, col + at * pitch);
                 row(bx, BWD ? piece_at<Q_>(dy, col + at * pitch) : bx, act);
@@ -562,31 +569,39 @@ __global__ __launch_bounds__(kStreamThreads, BWD && V == 8 ? 4 : 8) void gn_sums
         if (BWD) with_act(a.act, all);
         else all(std::integral_constant<int, SV_ACT_NONE>{});
     }
-    float *part = a.part + i * 2 * a.C, *first = sm + rpb * CB;
+    // rows together: across lanes where a wave holds whole rows (P a power of two), the rest through LDS
+    const bool lanes = lanes_share(P);
+    const int held = lanes ? NT / 64 : rpb, mine = lanes ? threadIdx.x >> 6 : r;
+    float *s1 = sm + held * CB, *first = s1 + held * CB;
+    if (lanes)
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        if (on)
+        for (int q = 0; q < 2; ++q)
 #pragma unroll
-            for (int e = 0; e < V; ++e) sm[r * CB + p * V + e] = acc[q][e];
-        __syncthreads();
-        for (int c = threadIdx.x; c < CB && slab * CB + c < a.C; c += NT) {
-            const int ch = slab * CB + c;
-            double t = 0.0;
-            for (int k = 0; k < rpb; ++k) t += (double)sm[k * CB + c];
-            float s = (float)t;
-            if (!BWD) {  // sums about the first row -> mean, and squares about it
-                if (q == 0) {
-                    s = s / (float)rows;
-                    first[c] = s;
-                    s += (float)((const T*)a.x)[(n * a.S + r0) * a.C + ch];
-                } else {
-                    s -= (float)rows * first[c] * first[c];
-                    s = s < 0.f ? 0.f : s;
-                }
-            }
-            part[q * a.C + ch] = s;
+            for (int e = 0; e < V; ++e) acc[q][e] = sum_stride(acc[q][e], P);
+    if (on && (!lanes || (threadIdx.x & 63) < P))
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            sm[mine * CB + p * V + e] = acc[0][e];
+            s1[mine * CB + p * V + e] = acc[1][e];
+            if (!BWD && r == 0) first[p * V + e] = mu[e];
         }
-        __syncthreads();
+    __syncthreads();
+    float* part = a.part + i * 2 * a.C + slab * CB;
+    for (int c = threadIdx.x; c < CB && slab * CB + c < a.C; c += NT) {
+        double u = 0.0, w = 0.0;
+        for (int k = 0; k < held; ++k) {
+            u += (double)sm[k * CB + c];
+            w += (double)s1[k * CB + c];
+        }
+        float s = (float)u, q = (float)w;
+        if (!BWD) {  // sums about the first row -> mean, and squares about it
+            const float m = s / (float)rows;
+            q -= s * m;
+            q = q < 0.f ? 0.f : q;
+            s = first[c] + m;
+        }
+        part[c] = s;
+        part[a.C + c] = q;
     }
 }
 
@@ -983,7 +998,8 @@ void launch_held(const GnArgs& a, const GnPlan& q, hipStream_t st) {
 template <typename T, bool BWD>
 void launch_streamed(const GnArgs& a, const GnPlan& q, hipStream_t st) {
     const int64_t main = a.N * q.chunks * q.slabs;
-    const size_t lds = ((size_t)(kStreamThreads / q.P) + 1) * q.CB * sizeof(float);  // at most 16 KB
+    const int held = lanes_share(q.P) ? kStreamThreads / 64 : kStreamThreads / q.P;
+    const size_t lds = (2 * (size_t)held + 1) * q.CB * sizeof(float);  // at most 24 KB
     const size_t lds_apply = 2 * ((size_t)q.CB / a.D + 2) * sizeof(float);
     with_piece<T>(q.V, [&](auto piece) {
         constexpr int V = decltype(piece)::value;

@@ -529,34 +529,20 @@ def batchnorm_sync_bwd_apply(x, dy, y_act, act_out, alpha_out: float, gamma, mea
           "sv_batchnorm_sync_bwd_apply")
 
 
-class _on:
-    """``with _on(x, ...) as stream``: the device all these tensors are on becomes the current one for the block; ``stream``
-    is its current stream."""
-
-    __slots__ = ("device", "guard")
-
-    def __init__(self, first, *rest):
-        dev = first.get_device()
-        for t in rest:
-            if t is not None and t.get_device() != dev:
-                raise ValueError(f"tensors on {first.device} and {t.device}: a launch takes tensors of one device")
-        if dev < 0:
-            raise _lib.SpectrumHipError(f"tensor is on {first.device}: the HIP path needs device tensors (no CPU fallback)")
-        self.device = dev
-        self.guard = None if dev == torch.cuda.current_device() else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch._C._cuda_getCurrentRawStream(self.device)  # torch.cuda.current_stream() without the object around it
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _here(first, *rest) -> Optional[int]:
+    """The current stream of the device that all these tensors are on, or None if that is not the current device."""
+    dev = first.get_device()
+    for t in rest:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors on {first.device} and {t.device}: a launch takes tensors of one device")
+    if dev < 0:
+        raise _lib.SpectrumHipError(f"tensor is on {first.device}: the HIP path needs device tensors (no CPU fallback)")
+    # torch.cuda.current_device() and current_stream() without the objects around them
+    return torch._C._cuda_getCurrentRawStream(dev) if dev == torch._C._cuda_getDevice() else None
 
 
 def _f32(t) -> Optional[int]:
-    """``_ptr`` of a float32 tensor whose device ``_on`` has seen."""
+    """``_ptr`` of a float32 tensor whose device ``_here`` has seen."""
     if t is None:
         return None
     return t.data_ptr() if t.dtype is torch.float32 and t.is_contiguous() else _ptr(t)
@@ -569,19 +555,20 @@ def groupnorm_workspace(n: int, s: int, c: int, groups: int) -> int:
 
 
 def _groupnorm_extents(x, like, gamma, beta, mean, rstd, groups: int):
-    if x.dim() < 2 or like.shape != x.shape:
+    shape = x.shape
+    if len(shape) < 2 or like.shape != shape:
         raise ValueError(f"groupnorm: [N, ..., C] tensors of one shape, not {tuple(x.shape)} and {tuple(like.shape)}")
-    n, c = x.shape[0], x.shape[-1]
-    s = 1
-    for d in x.shape[1:-1]:
+    n, c, s = shape[0], shape[-1], 1
+    for d in shape[1:-1]:
         s *= d
     if groups < 1 or c % groups:
         raise ValueError(f"groupnorm: {c} channels do not split into {groups} groups")
     if gamma.numel() != c or beta.numel() != c:
         raise ValueError(f"groupnorm: gamma / beta must have the {c} channels' size")
-    if (mean is None) != (rstd is None):
-        raise ValueError("groupnorm: saved mean and rstd go together")
-    if mean is not None and (mean.numel() != n * groups or rstd.numel() != n * groups):
+    if mean is None or rstd is None:
+        if mean is not rstd:
+            raise ValueError("groupnorm: saved mean and rstd go together")
+    elif mean.numel() != n * groups or rstd.numel() != n * groups:
         raise ValueError("groupnorm: saved statistics must be [N][groups]")
     return n, s, c
 
@@ -590,10 +577,12 @@ def groupnorm_act_fwd(x, gamma, beta, y, save_mean, save_rstd, groups: int, eps:
     """y = act((x - mean) * rstd * gamma + beta), mean and rstd over each sample's channel groups; x, y [N, ..., C] float32 or
     bfloat16, everything else float32.  save_mean / save_rstd [N, groups]: for the backward call; both may be None."""
     n, s, c = _groupnorm_extents(x, y, gamma, beta, save_mean, save_rstd, groups)
-    with _on(x, gamma, beta, y, save_mean, save_rstd, ws) as stream:
-        check(lib.sv_groupnorm_act_fwd(_aptr(x), _f32(gamma), _f32(beta), _aptr(y, x, "y"), _f32(save_mean), _f32(save_rstd),
-                                       n, s, c, groups, eps, ACT[act], alpha, *_ws_args(ws), _dt(x), stream),
-              "sv_groupnorm_act_fwd")
+    stream = _here(x, gamma, beta, y, save_mean, save_rstd, ws)
+    if stream is None:
+        with torch.cuda.device(x.device):
+            return groupnorm_act_fwd(x, gamma, beta, y, save_mean, save_rstd, groups, eps, act, alpha, ws)
+    check(lib.sv_groupnorm_act_fwd(_aptr(x), _f32(gamma), _f32(beta), _aptr(y, x, "y"), _f32(save_mean), _f32(save_rstd), n, s,
+                                   c, groups, eps, ACT[act], alpha, *_ws_args(ws), _dt(x), stream), "sv_groupnorm_act_fwd")
 
 
 def groupnorm_act_bwd(x, dy, gamma, beta, save_mean, save_rstd, dx, dgamma, dbeta, accumulate: bool, groups: int, act,
@@ -604,10 +593,13 @@ def groupnorm_act_bwd(x, dy, gamma, beta, save_mean, save_rstd, dx, dgamma, dbet
     n, s, c = _groupnorm_extents(x, dy, gamma, beta, save_mean, save_rstd, groups)
     if dgamma.numel() != c or dbeta.numel() != c:
         raise ValueError(f"groupnorm: dgamma / dbeta must have the {c} channels' size")
-    with _on(x, dy, gamma, beta, save_mean, save_rstd, dx, dgamma, dbeta, ws) as stream:
-        check(lib.sv_groupnorm_act_bwd(_aptr(x), _aptr(dy, x, "dy"), _f32(gamma), _f32(beta), _f32(save_mean), _f32(save_rstd),
-                                       _aptr(dx, x, "dx"), _f32(dgamma), _f32(dbeta), int(accumulate), n, s, c, groups,
-                                       ACT[act], alpha, *_ws_args(ws), _dt(x), stream), "sv_groupnorm_act_bwd")
+    stream = _here(x, dy, gamma, beta, save_mean, save_rstd, dx, dgamma, dbeta, ws)
+    if stream is None:
+        with torch.cuda.device(x.device):
+            return groupnorm_act_bwd(x, dy, gamma, beta, save_mean, save_rstd, dx, dgamma, dbeta, accumulate, groups, act, alpha, ws)
+    check(lib.sv_groupnorm_act_bwd(_aptr(x), _aptr(dy, x, "dy"), _f32(gamma), _f32(beta), _f32(save_mean), _f32(save_rstd),
+                                   _aptr(dx, x, "dx"), _f32(dgamma), _f32(dbeta), int(accumulate), n, s, c, groups, ACT[act],
+                                   alpha, *_ws_args(ws), _dt(x), stream), "sv_groupnorm_act_bwd")
 
 
 def concat_channels_fwd(a, b, y, rows, ca, cb):
@@ -824,11 +816,14 @@ def adamw_step(plan: AdamWPlan, state, lr0, beta1, beta2, eps, decay_steps=0, de
     of the random bits that round 8-bit moments."""
     if state.numel() < 3:
         raise ValueError("adamw: the step state is int64[3]")
-    with _on(plan._image, state) as stream:
-        check(lib.sv_adamw_step(plan._image.data_ptr(), plan.n_chunks, plan.state_bits,
-                                _ptr(state, torch.int64), lr0, beta1, beta2, eps, int(decay_steps or 0), decay_rate,
-                                int(staircase), grad_scale, clip_norm, seed, int(zero_grad), plan._ws.data_ptr(),
-                                plan._ws.numel(), stream), "sv_adamw_step")
+    stream = _here(plan._image, state)
+    if stream is None:
+        with torch.cuda.device(plan.device):
+            return adamw_step(plan, state, lr0, beta1, beta2, eps, decay_steps, decay_rate, staircase, grad_scale, clip_norm, seed,
+                              zero_grad)
+    check(lib.sv_adamw_step(plan._image.data_ptr(), plan.n_chunks, plan.state_bits, _ptr(state, torch.int64), lr0, beta1, beta2,
+                            eps, int(decay_steps or 0), decay_rate, int(staircase), grad_scale, clip_norm, seed, int(zero_grad),
+                            plan._ws.data_ptr(), plan._ws.numel(), stream), "sv_adamw_step")
 
 
 def adamw_decode(codes, exponents, out, second: bool):
@@ -837,9 +832,12 @@ def adamw_decode(codes, exponents, out, second: bool):
     n = codes.numel()
     if out.numel() != n or exponents.numel() != -(-n // ADAMW_BLOCK):
         raise ValueError("adamw_decode: sizes differ")
-    with _on(codes, exponents, out) as stream:
-        check(lib.sv_adamw_decode(_ptr(codes, torch.uint8), _ptr(exponents, torch.uint8), _ptr(out), n, int(bool(second)),
-                                  stream), "sv_adamw_decode")
+    stream = _here(codes, exponents, out)
+    if stream is None:
+        with torch.cuda.device(codes.device):
+            return adamw_decode(codes, exponents, out, second)
+    check(lib.sv_adamw_decode(_ptr(codes, torch.uint8), _ptr(exponents, torch.uint8), _ptr(out), n, int(bool(second)), stream),
+          "sv_adamw_decode")
 
 
 # --------------------------------------------------------------------------- batching helpers
