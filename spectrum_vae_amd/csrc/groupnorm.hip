@@ -139,7 +139,8 @@ struct GnArgs {
     float* rstd;
     void* out;      // y or dx
     float* part;    // held, backward: [N][2][C]; streamed: [N][chunks][2][C]
-    float* folded;  // streamed: [N][2][C], or null where the chunks are few
+    float* folded;  // streamed: [N][2][C], the chunks joined by gn_fold_k, or
+    float* groups;  //           [N][chunks][2][G], the chunks' values of whole groups, joined in the second pass (else null)
     float* dgamma;
     float* dbeta;
     int64_t N, S;
@@ -496,7 +497,7 @@ __host__ __device__ __forceinline__ bool lanes_share(int P) { return P <= 64 && 
 // Eight workgroups a CU: 2048 of them are resident at once (with eight bf16 channels a thread, backward, half of them).
 template <typename T, int V, bool BWD>
 __global__ __launch_bounds__(kStreamThreads, BWD && V == 8 ? 4 : 8) void gn_sums_k(GnArgs a) {
-    extern __shared__ float sm[];  // [2][rows at a time, or waves][channels of a slab] | [channels] of the first row
+    extern __shared__ float sm[];  // [2][rows at a time, or waves][channels of a slab] | [3][channels]
     constexpr int NT = kStreamThreads, U = BWD ? 2 : V == 8 ? 4 : 8;  // pieces of each tensor in flight
     const int slab = (int)(blockIdx.x % a.slabs);
     const int64_t i = blockIdx.x / a.slabs, n = i / a.chunks, chunk = i % a.chunks;
@@ -600,8 +601,45 @@ __global__ __launch_bounds__(kStreamThreads, BWD && V == 8 ? 4 : 8) void gn_sums
             q = q < 0.f ? 0.f : q;
             s = first[c] + m;
         }
-        part[c] = s;
-        part[a.C + c] = q;
+        if (BWD || a.groups == nullptr) {
+            part[c] = s;
+            part[a.C + c] = q;
+        }
+        if (a.groups != nullptr) {
+            first[CB + c] = s;
+            first[2 * CB + c] = q;
+        }
+    }
+    if (a.groups == nullptr) return;
+    // one slab: the groups' values of this chunk
+    __syncthreads();
+    const float *chs = first + CB, *chq = first + 2 * CB;
+    const int share = lanes_for(a.D), lane = threadIdx.x & (share - 1);
+    for (int g = threadIdx.x / share; g < a.G; g += NT / share) {
+        double s = 0.0, q = 0.0;
+        const double piv = BWD ? 0.0 : (double)chs[g * a.D];
+        for (int c = g * a.D + lane; c < (g + 1) * a.D; c += share) {
+            if (BWD) {
+                s += (double)a.gamma[c] * (double)chs[c];
+                q += (double)a.gamma[c] * (double)chq[c];
+            } else {
+                const double d = (double)chs[c] - piv;
+                s += d;
+                q += (double)chq[c] + (double)rows * d * d;
+            }
+        }
+        for (int o = share >> 1; o > 0; o >>= 1) {
+            s += __shfl_xor(s, o, 64);
+            q += __shfl_xor(q, o, 64);
+        }
+        if (lane == 0) {
+            if (!BWD) {
+                q -= (double)rows / (double)a.D * s * s;
+                s = piv + s / (double)a.D;
+            }
+            a.groups[(i * 2 + 0) * a.G + g] = (float)s;
+            a.groups[(i * 2 + 1) * a.G + g] = !BWD && q < 0.0 ? 0.f : (float)q;
+        }
     }
 }
 
@@ -707,24 +745,27 @@ __global__ __launch_bounds__(1024) void gn_param_fold_k(const float* __restrict_
     fold_params<1024>(part, parts, C, blockIdx.x * 16 + (threadIdx.x & 15), dgamma, dbeta, accumulate, red);
 }
 
-// The two values of a group from f, its channels' values for `parts` parts of a sample with `rows` rows each (the last with the
-// rest), summed by `lanes` neighbouring lanes.  Forward: mean, rstd.  Backward: mean_g(gz), mean_g(gz xhat).
+// The two values of group g of sample n from its D channels' joined ones (a.folded) or from its chunks' ones (a.groups), summed by
+// `lanes` neighbouring lanes.  Forward: mean, rstd.  Backward: mean_g(gz), mean_g(gz xhat).
 template <bool BWD>
-__device__ __forceinline__ void group_values(const GnArgs& a, const float* f, int parts, int64_t rows, int g, int lane, int lanes,
-                                             float& u, float& v) {
+__device__ __forceinline__ void group_values(const GnArgs& a, int64_t n, int g, int lane, int lanes, float& u, float& v) {
+    const bool whole = a.groups != nullptr;
+    const int terms = whole ? a.chunks : a.D, pitch = whole ? a.G : a.C;  // a term's two values are `pitch` apart
+    const int64_t step = whole ? 2 * a.G : 1;                             // two terms
+    const float* f = whole ? a.groups + n * a.chunks * 2 * a.G + g : a.folded + n * 2 * a.C + g * a.D;
+    const double piv = BWD ? 0.0 : (double)f[0];
     double s = 0.0, q = 0.0;
-    const double piv = BWD ? 0.0 : (double)f[g * a.D];
-    for (int i = lane; i < parts * a.D; i += lanes) {
-        const int k = parts == 1 ? 0 : i / a.D, c = g * a.D + i - k * a.D;
-        const double x = (double)f[(int64_t)k * 2 * a.C + c], y = (double)f[(int64_t)k * 2 * a.C + a.C + c];
+#pragma unroll 4
+    for (int i = lane; i < terms; i += lanes) {
+        const double x = (double)f[i * step], y = (double)f[i * step + pitch];
         if (BWD) {
-            const double w = (double)a.gamma[c];
+            const double w = whole ? 1.0 : (double)a.gamma[g * a.D + i];
             s += w * x;
             q += w * y;
-        } else {
-            const double r = (double)((k + 1) * rows < a.S ? rows : a.S - k * rows), d = x - piv;
-            s += r * d;
-            q += y + r * d * d;
+        } else {  // means and squares about them, of r values each
+            const double r = whole ? (double)a.D * (double)((i + 1) * a.rows < a.S ? a.rows : a.S - i * a.rows) : (double)a.S;
+            s += r * (x - piv);
+            q += y + r * (x - piv) * (x - piv);
         }
     }
     for (int o = lanes >> 1; o > 0; o >>= 1) {
@@ -746,26 +787,25 @@ template <typename T, int V, bool BWD>
 __global__ __launch_bounds__(kStreamThreads, BWD && V == 8 ? 4 : 8) void gn_apply_k(GnArgs a) {
     extern __shared__ float gv[];  // [2][groups that the slab touches]
     constexpr int NT = kStreamThreads, U = BWD || V == 8 ? 2 : 4;
-    const int64_t main = a.N * a.chunks * a.slabs;
-    const bool joined = a.folded != nullptr;  // by gn_fold_k; else from the chunks' sums here
-    if (BWD && blockIdx.x >= main) {  // the last workgroups: dgamma, dbeta
+    const int extra = BWD ? (a.C + 15) / 16 : 0;
+    if (BWD && (int)blockIdx.x < extra) {  // the first workgroups: dgamma, dbeta
         __shared__ double red[2 * (NT / 16) * 16];
-        fold_params<NT>(joined ? a.folded : a.part, joined ? a.N : a.N * a.chunks, a.C,
-                        (int)(blockIdx.x - main) * 16 + (threadIdx.x & 15), a.dgamma, a.dbeta, a.accumulate, red);
+        const bool joined = a.groups == nullptr;
+        fold_params<NT>(joined ? a.folded : a.part, joined ? a.N : a.N * a.chunks, a.C, blockIdx.x * 16 + (threadIdx.x & 15),
+                        a.dgamma, a.dbeta, a.accumulate, red);
         return;
     }
     // last chunk first: what the statistics pass read last is what the caches still hold
-    const int64_t bid = main - 1 - blockIdx.x;
+    const int64_t bid = (int64_t)gridDim.x - 1 - blockIdx.x;
     const int slab = (int)(bid % a.slabs);
     const int64_t i = bid / a.slabs, n = i / a.chunks, chunk = i % a.chunks;
     const int first = slab * a.CB, P = a.P, rpb = NT / P;
     const int last = first + a.CB < a.C ? first + a.CB : a.C;
     const int g0 = first / a.D, g1 = (last - 1) / a.D + 1, gs = g1 - g0;
-    const float* f = joined ? a.folded + n * 2 * a.C : a.part + n * a.chunks * 2 * a.C;
-    const int parts = joined ? 1 : a.chunks, lanes = lanes_for(parts * a.D);
+    const int lanes = lanes_for(a.groups != nullptr ? a.chunks : a.D);
     for (int g = g0 + threadIdx.x / lanes; g < g1; g += NT / lanes) {
         float u, v;
-        group_values<BWD>(a, f, parts, joined ? a.S : a.rows, g, threadIdx.x % lanes, lanes, u, v);
+        group_values<BWD>(a, n, g, threadIdx.x % lanes, lanes, u, v);
         if (threadIdx.x % lanes == 0) {
             gv[g - g0] = u;
             gv[gs + g - g0] = v;
@@ -852,17 +892,19 @@ int piece_of(int C, int size, uintptr_t bits) {
     return v;
 }
 
-// Chunks of the streamed form: about 2048 workgroups in all, what the chip holds at once, and at least 8 rows a thread.
-void plan_streamed(GnPlan& q, int64_t N, int64_t S, int C) {
+// Chunks of the streamed form: `deep` rows a thread, and at most 2048 workgroups, what the chip holds at once; 512 of them, two a CU,
+// come first, down to two rows a thread.
+void plan_streamed(GnPlan& q, int64_t N, int64_t S, int C, int deep) {
     const int P = C / q.V < kStreamThreads ? C / q.V : kStreamThreads;
     q.K = 0;
     q.NT = kStreamThreads;
     q.P = P;
     q.CB = P * q.V;
     q.slabs = (int)ceil_div(C, q.CB);
-    const int64_t least = 8 * (kStreamThreads / P);
-    int64_t chunks = ceil_div(2048, N * q.slabs);
-    if (chunks > ceil_div(S, least)) chunks = ceil_div(S, least);
+    const auto lesser = [](int64_t x, int64_t y) { return x < y ? x : y; };
+    const int64_t parts = N * q.slabs, rows = ceil_div(S, kStreamThreads / P);  // rows of one thread
+    const int64_t few = lesser(ceil_div(rows, 2), ceil_div(512, parts)), many = lesser(ceil_div(rows, deep), ceil_div(2048, parts));
+    const int64_t chunks = few < many ? many : few;
     q.rows = ceil_div(S, chunks);
     const int64_t fit = 0xffffffffll / (4 * (int64_t)C);  // a chunk's offsets have 32 bits
     if (q.rows > fit) q.rows = fit;
@@ -915,24 +957,27 @@ GnPlan gn_plan(int64_t N, int64_t S, int C, int G, int size, uintptr_t bits, boo
         q.groups = groups;
         return q;
     }
-    plan_streamed(q, N, S, C);
+    // Sixteen rows a thread for two tensors and for narrow pieces, else eight (33 MB of bf16, 64 samples of 90x90x32: backward 35.8 us
+    // against 37.8, forward 29.0 against 27.7; 100 samples of 30x31x45 bf16 forward 17.8 against 22.2).
+    plan_streamed(q, N, S, C, bwd || q.V * size < 8 ? 16 : 8);
     return q;
 }
 
-// workspace: [N][2][C] folded sums | [N][chunks][2][C] partial sums, the chunks the most of any type and alignment.
+// workspace: [N][2][C] folded sums | [N][chunks][2][C] channels' and [N][chunks][2][G] groups' partial sums, the chunks the most of
+// any type and alignment.
 int64_t gn_most_chunks(int64_t N, int64_t S, int C) {
     int64_t most = 1;
     for (int v = 1; v <= 8; v *= 2)
         if (C % v == 0) {
             GnPlan q{};
             q.V = v;
-            plan_streamed(q, N, S, C);
+            plan_streamed(q, N, S, C, 8);
             if (q.chunks > most) most = q.chunks;
         }
     return most;
 }
-size_t gn_ws_bytes(int64_t N, int64_t S, int C) {
-    return (size_t)N * 2 * C * (1 + (size_t)gn_most_chunks(N, S, C)) * sizeof(float);
+size_t gn_ws_bytes(int64_t N, int64_t S, int C, int G) {
+    return (size_t)N * 2 * (C + (size_t)(C + G) * gn_most_chunks(N, S, C)) * sizeof(float);
 }
 
 int gn_check(const char* who, int64_t N, int64_t S, int C, int G, int act, void* ws, size_t ws_bytes) {
@@ -943,7 +988,7 @@ int gn_check(const char* who, int64_t N, int64_t S, int C, int G, int act, void*
     SV_REQUIRE(act >= SV_ACT_NONE && act <= SV_ACT_SIGMOID, "%s: activation %d unknown", who, act);
     if (N == 0) return SV_OK;
     SV_REQUIRE(N <= (1 << 24) && N * C <= 0x3fffffff, "%s: too many samples", who);
-    const size_t need = gn_ws_bytes(N, S, C);
+    const size_t need = gn_ws_bytes(N, S, C, G);
     if (ws == nullptr || ws_bytes < need) return fail(SV_E_WORKSPACE, "%s: workspace %zu bytes < required %zu", who, ws_bytes, need);
     return SV_OK;
 }
@@ -999,12 +1044,12 @@ template <typename T, bool BWD>
 void launch_streamed(const GnArgs& a, const GnPlan& q, hipStream_t st) {
     const int64_t main = a.N * q.chunks * q.slabs;
     const int held = lanes_share(q.P) ? kStreamThreads / 64 : kStreamThreads / q.P;
-    const size_t lds = (2 * (size_t)held + 1) * q.CB * sizeof(float);  // at most 24 KB
+    const size_t lds = (2 * (size_t)held + 3) * q.CB * sizeof(float);  // at most 40 KB
     const size_t lds_apply = 2 * ((size_t)q.CB / a.D + 2) * sizeof(float);
     with_piece<T>(q.V, [&](auto piece) {
         constexpr int V = decltype(piece)::value;
         hipLaunchKernelGGL((gn_sums_k<T, V, BWD>), dim3((unsigned)main), dim3(kStreamThreads), lds, st, a);
-        if (a.folded != nullptr)
+        if (a.groups == nullptr)
             hipLaunchKernelGGL((gn_fold_k<BWD>), dim3((unsigned)a.N, (unsigned)ceil_div(a.C, 16)), dim3(1024), 0, st, a);
         hipLaunchKernelGGL((gn_apply_k<T, V, BWD>), dim3((unsigned)(main + (BWD ? ceil_div(a.C, 16) : 0))),
                            dim3(kStreamThreads), lds_apply, st, a);
@@ -1030,8 +1075,10 @@ void launch(GnArgs& a, void* workspace, hipStream_t st) {
                                a.N, a.C, a.accumulate);
     } else {
         a.part = a.folded + a.N * 2 * a.C;
-        // few chunks: the second pass joins them itself, which saves a launch (19 -> 14 us at 37 samples of 31x29x90, for example)
-        if (a.chunks <= 32 && a.chunks * a.D <= 512 && (!BWD || a.N * a.chunks <= 256)) a.folded = nullptr;
+        // Few chunks and whole groups in a slab: the second pass joins the groups' values itself, which saves a launch (32 samples of
+        // 128x128x32 bf16 forward 28.2 -> 26.9 us, backward 38.1 -> 37.1; at two samples of 512x512 and 1024 chunks each 29.7 -> 38.3).
+        // Backward, its first workgroups also add the channels' sums of all chunks.
+        if (q.slabs == 1 && q.chunks <= 64 && (!BWD || a.N * q.chunks <= 2048)) a.groups = a.part + a.N * q.chunks * 2 * a.C;
         launch_streamed<T, BWD>(a, q, st);
     }
 }
@@ -1045,7 +1092,7 @@ extern "C" {
 
 size_t sv_groupnorm_workspace_bytes(int64_t N, int64_t S, int C, int groups) {
     if (N <= 0 || S <= 0 || C <= 0 || C > kGnMaxC || groups < 1 || C % groups) return 0;
-    return gn_ws_bytes(N, S, C);
+    return gn_ws_bytes(N, S, C, groups);
 }
 
 int sv_groupnorm_act_fwd(const void* x, const float* gamma, const float* beta, void* y, float* save_mean, float* save_rstd,
