@@ -922,7 +922,9 @@ GnPlan gn_plan(int64_t N, int64_t S, int C, int G, int size, uintptr_t bits, boo
     // whose phases overlap.  A sample of more rows in 64-byte rows with 512 threads before 128-byte ones with 1024, of which a CU
     // holds one (512 samples of 32x32x64 bf16 forward 40 against 47 us, f32 backward 92 against 104) - but for the f32 forward
     // pass of whole groups, of which it holds two (1024 samples of 32x32x64 111 against 125 us).  Below 64 bytes a
-    // row the streamed form is faster.
+    // row the streamed form is faster, and where fewer than 64 workgroups would hold 4096 pieces and more each: it spreads them (16
+    // samples of 40x40x48 bf16 backward 12.8 against 17.9 us, 8 of 64x64x64 forward 12.9 against 18.8; from 128 workgroups on
+    // the held form wins, 32 samples of 32x32x64 f32 forward 11.2 against 12.5).
     struct Form {
         int row, K, NT;
         bool two;
@@ -946,7 +948,7 @@ GnPlan gn_plan(int64_t N, int64_t S, int C, int G, int size, uintptr_t bits, boo
         const bool groups = log2_of(D) >= 0 && D >= q.V && P == 1 << log_q && P <= 64 && piece >= 8;
         if (cb > kHeldMaxC || 1 << log_q > f.NT || f.K * piece > most || S > (int64_t)f.K * f.NT >> log_q ||
             f.NT / (log_q < 6 ? 64 : 1 << log_q) * cb > kHeldSlots || (f.two && !(groups && size == 4 && !bwd)) ||
-            !held_compiled(bwd, size, piece, f.K, f.NT, groups))
+            !held_compiled(bwd, size, piece, f.K, f.NT, groups) || (f.K * f.NT >= 4096 && N * ceil_div(C, cb) < 64))
             continue;
         q.K = f.K;
         q.NT = f.NT;
