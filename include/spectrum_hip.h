@@ -17,8 +17,8 @@
  *    (kh,kw,Cout,Cin), Dense kernels (in,out): the tf.keras layouts;
  *  - `dtype` selects the storage type of activations, filters and activation gradients: SV_F32 everywhere, SV_BF16 in
  *    the strided / transposed conv family (sv_conv2d_{fwd,dgrad,wgrad}[_ws], sv_conv2d_transpose_*, sv_conv2d_wgrad_static),
- *    sv_act_*, sv_bias_grad, sv_batchnorm_*, sv_concat_channels_*, sv_axpy, sv_mask_input_dt and the losses (prediction
- *    and its gradient; targets, masks and weights stay f32).  Sums are always f32; biases, BatchNorm parameters and
+ *    sv_act_*, sv_bias_grad, sv_batchnorm_*, sv_groupnorm_*, sv_concat_channels_*, sv_axpy, sv_mask_input_dt and the losses (prediction
+ *    and its gradient; targets, masks and weights stay f32).  Sums are always f32; biases, normalisation parameters and
  *    statistics, loss values and every kernel / bias gradient (dw, db, dgamma, dbeta) are f32 in both modes: the master
  *    weights and the Adam step stay f32, a bf16 model keeps a bf16 copy of its filters (sv_cast_f32_bf16).
  */
@@ -388,7 +388,8 @@ int sv_batchnorm_sync_bwd_apply(const void* x, const void* dy, const void* y_act
  *  - save_mean / save_rstd [N, groups], f32: what the backward call needs; both may be NULL (inference).
  *  - backward: dgamma / dbeta (+)= the sums over N and S, formed in a fixed order.  The activation's slope is recomputed
  *    from x; at 0 it is that of the negative side.
- *  - tensors need no alignment beyond their elements'; outputs must not overlap inputs.
+ *  - tensors need no alignment beyond their elements'.  y may be x, and dx may be dy or x; otherwise outputs must not overlap
+ *    inputs.
  *  workspace: sv_groupnorm_workspace_bytes, 16-byte aligned, for either direction. */
 size_t sv_groupnorm_workspace_bytes(int64_t N, int64_t S, int C, int groups);
 int sv_groupnorm_act_fwd(const void* x, const float* gamma, const float* beta, void* y, float* save_mean, float* save_rstd,
@@ -530,7 +531,7 @@ int sv_adam_keras_apply(float* theta, float* grad, float* m, float* v, int64_t n
  *      alpha as in sv_adam_keras_step, per element of every tensor:
  *        g *= s;  m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2;  theta -= lr weight_decay theta;  theta -= alpha m/(sqrt(v)+eps)
  *      s = grad_scale, or with clip_norm > 0 grad_scale * clip_norm / max(clip_norm, norm), norm = grad_scale * the 2-norm of all
- *      gradients (one more launch; not finite: everything becomes NaN).
+ *      gradients (one more launch; not finite: everything becomes NaN).  eps is at least 1e-12.
  *  sv_adamw_tensor: one tensor.  n may be 0; weight_decay is its own; theta_bf16 may be NULL (a copy written with theta).
  *      state_bits 32: m and v are float[n], m_exp / v_exp unused.
  *      state_bits 8: m and v are uint8[n], m_exp / v_exp uint8[ceil(n / 256)], all zero at the start.  A block of 256 elements

@@ -507,7 +507,9 @@ int sv_adamw_step(void* plan, int64_t n_chunks, int state_bits, int64_t* step_st
     SV_REQUIRE((uintptr_t)plan % 128 == 0 && (uintptr_t)step_state % 8 == 0, "sv_adamw_step: plan must be 128-byte, state 8-byte aligned");
     SV_REQUIRE(state_bits == 8 || state_bits == 32, "sv_adamw_step: moments have 8 or 32 bits, not %d", state_bits);
     SV_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "sv_adamw_step: betas out of range");
-    SV_REQUIRE(eps > 0.f && clip_norm >= 0.f && (decay_steps <= 0 || decay_rate > 0.0), "sv_adamw_step: epsilon and the decay rate must be positive, the clip not negative");
+    // the step's root takes second moments below 1.2e-38 as 0, which is 1e-19 in it: nothing next to such an epsilon
+    SV_REQUIRE(eps >= 1e-12f, "sv_adamw_step: epsilon must be at least 1e-12");
+    SV_REQUIRE(clip_norm >= 0.f && (decay_steps <= 0 || decay_rate > 0.0), "sv_adamw_step: the decay rate must be positive, the clip not negative");
     SV_REQUIRE(clip_norm == 0.f || (workspace != nullptr && (uintptr_t)workspace % 8 == 0), "sv_adamw_step: clipping needs a workspace");
     if (clip_norm > 0.f && workspace_bytes < sv_adamw_workspace_bytes())
         return fail(SV_E_WORKSPACE, "sv_adamw_step: workspace %zu bytes < required %zu", workspace_bytes, sv_adamw_workspace_bytes());

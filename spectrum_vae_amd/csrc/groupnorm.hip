@@ -1059,7 +1059,7 @@ void launch_streamed(const GnArgs& a, const GnPlan& q, hipStream_t st) {
 }
 
 template <typename T, bool BWD>
-void launch(GnArgs& a, void* workspace, hipStream_t st) {
+int launch(const char* who, GnArgs& a, void* workspace, hipStream_t st) {
     const uintptr_t bits = (uintptr_t)a.x | (uintptr_t)a.out | (uintptr_t)a.dy;
     const GnPlan q = gn_plan(a.N, a.S, a.C, a.G, sizeof(T), bits, BWD);
     a.CB = q.CB;
@@ -1069,6 +1069,9 @@ void launch(GnArgs& a, void* workspace, hipStream_t st) {
     a.rows = q.rows;
     a.chunks = q.chunks;
     a.folded = (float*)workspace;
+    const int64_t grid = q.K > 0 ? held_grid(a.N, q.slabs) : a.N * q.chunks * q.slabs + ceil_div(a.C, 16);
+    const int64_t threads = q.K > 0 ? grid * q.NT : grid * kStreamThreads;  // (gn_fold_k: N * 1024)
+    SV_REQUIRE(threads <= 0xffffffffll && (q.K > 0 || a.N < (1 << 22)), "%s: too many samples for one launch", who);
     if (q.K > 0) {
         a.part = (float*)workspace;
         launch_held<T, BWD>(a, q, st);
@@ -1083,6 +1086,7 @@ void launch(GnArgs& a, void* workspace, hipStream_t st) {
         if (q.slabs == 1 && q.chunks <= 64 && (!BWD || a.N * q.chunks <= 2048)) a.groups = a.part + a.N * q.chunks * 2 * a.C;
         launch_streamed<T, BWD>(a, q, st);
     }
+    return check_launch(who);
 }
 
 }  // namespace
@@ -1103,6 +1107,7 @@ int sv_groupnorm_act_fwd(const void* x, const float* gamma, const float* beta, v
     SV_F32_OR_BF16(dtype, "sv_groupnorm_act_fwd");
     int rc = gn_check("sv_groupnorm_act_fwd", N, S, C, groups, act, workspace, workspace_bytes);
     if (rc) return rc;
+    SV_REQUIRE(eps >= 0.f, "sv_groupnorm_act_fwd: epsilon must not be negative");
     SV_REQUIRE((save_mean == nullptr) == (save_rstd == nullptr), "sv_groupnorm_act_fwd: save_mean and save_rstd go together");
     if (N == 0) return SV_OK;
     SV_REQUIRE(x && gamma && beta && y, "sv_groupnorm_act_fwd: null tensor");
@@ -1121,9 +1126,8 @@ int sv_groupnorm_act_fwd(const void* x, const float* gamma, const float* beta, v
     a.eps = eps;
     a.act = act;
     a.alpha = alpha;
-    if (dtype == SV_F32) launch<float, false>(a, workspace, to_stream(stream));
-    else launch<__bf16, false>(a, workspace, to_stream(stream));
-    return check_launch("sv_groupnorm_act_fwd");
+    const auto run = dtype == SV_F32 ? launch<float, false> : launch<__bf16, false>;
+    return run("sv_groupnorm_act_fwd", a, workspace, to_stream(stream));
 }
 
 int sv_groupnorm_act_bwd(const void* x, const void* dy, const float* gamma, const float* beta, const float* save_mean,
@@ -1159,9 +1163,8 @@ int sv_groupnorm_act_bwd(const void* x, const void* dy, const float* gamma, cons
     a.D = C / groups;
     a.act = act;
     a.alpha = alpha;
-    if (dtype == SV_F32) launch<float, true>(a, workspace, st);
-    else launch<__bf16, true>(a, workspace, st);
-    return check_launch("sv_groupnorm_act_bwd");
+    const auto run = dtype == SV_F32 ? launch<float, true> : launch<__bf16, true>;
+    return run("sv_groupnorm_act_bwd", a, workspace, st);
 }
 
 }  // extern "C"

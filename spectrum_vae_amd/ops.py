@@ -575,7 +575,8 @@ def _groupnorm_extents(x, like, gamma, beta, mean, rstd, groups: int):
 
 def groupnorm_act_fwd(x, gamma, beta, y, save_mean, save_rstd, groups: int, eps: float, act, alpha: float, ws):
     """y = act((x - mean) * rstd * gamma + beta), mean and rstd over each sample's channel groups; x, y [N, ..., C] float32 or
-    bfloat16, everything else float32.  save_mean / save_rstd [N, groups]: for the backward call; both may be None."""
+    bfloat16, everything else float32; y may be x.  save_mean / save_rstd [N, groups]: for the backward call; both may be
+    None."""
     n, s, c = _groupnorm_extents(x, y, gamma, beta, save_mean, save_rstd, groups)
     stream = _here(x, gamma, beta, y, save_mean, save_rstd, ws)
     if stream is None:
@@ -587,7 +588,8 @@ def groupnorm_act_fwd(x, gamma, beta, y, save_mean, save_rstd, groups: int, eps:
 
 def groupnorm_act_bwd(x, dy, gamma, beta, save_mean, save_rstd, dx, dgamma, dbeta, accumulate: bool, groups: int, act,
                       alpha: float, ws):
-    """Backward of ``groupnorm_act_fwd`` from its input (its output is not needed): dx, and dgamma / dbeta (+)= their sums."""
+    """Backward of ``groupnorm_act_fwd`` from its input (its output is not needed): dx, and dgamma / dbeta (+)= their sums.
+    dx may be dy or x."""
     if save_mean is None or dx.shape != x.shape:
         raise ValueError("groupnorm: the backward call needs the saved statistics and dx of x's shape")
     n, s, c = _groupnorm_extents(x, dy, gamma, beta, save_mean, save_rstd, groups)

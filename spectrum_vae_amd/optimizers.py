@@ -154,6 +154,8 @@ class AdamW(Adam):
         super().__init__(learning_rate, beta_1, beta_2, epsilon)
         if weight_decay < 0:
             raise ValueError("weight_decay must not be negative")
+        if epsilon < 1e-12:
+            raise ValueError("epsilon must be at least 1e-12")
         if global_clipnorm is not None and global_clipnorm <= 0:
             raise ValueError("global_clipnorm must be positive")
         if state_bits not in (8, 32):

@@ -274,6 +274,89 @@ def test_a_plan_of_many_tensors_and_refusals_on_the_device():
         ops.adamw_step(plan, state[:2], 1e-3, 0.9, 0.999, 1e-7)
 
 
+@pytest.mark.parametrize("clip", [0.0, 0.5])
+@pytest.mark.parametrize("bits,sizes", [(32, [2_000_001]), (8, [2_000_001]), (32, [9_000_000, 3, 700_001]), (8, [9_000_000, 3, 700_001]),
+                                        (32, [20_000_003, 70]), (8, [30_000_003, 70])])
+def test_large_tensors_by_samples(bits, sizes, clip):
+    """More entries than workgroups, one to four workgroups an entry, and more bytes than the caches hold; blocks of 256 drawn from
+    all over, the first and the last (incomplete) ones among them, against the oracle."""
+    from spectrum_vae_amd import ops
+    rng = np.random.default_rng(sum(sizes) + bits)
+    g = torch.Generator(device="cuda").manual_seed(bits)
+    randn = lambda n: torch.randn(n, device="cuda", generator=g)  # noqa: E731
+    theta, grads = [0.1 * randn(n) for n in sizes], [1e-2 * randn(n) for n in sizes]
+    lp = [torch.empty(n, dtype=torch.bfloat16, device="cuda") for n in sizes]
+    blocks = [-(-n // 256) for n in sizes]
+    if bits == 8:
+        m, v = ([torch.randint(0, 256, (n,), dtype=torch.uint8, device="cuda", generator=g) for n in sizes] for _ in range(2))
+        me, ve = ([torch.randint(115, 121, (b,), dtype=torch.uint8, device="cuda", generator=g) for b in blocks] for _ in range(2))
+    else:
+        m, v, me, ve = [1e-3 * randn(n) for n in sizes], [1e-4 * randn(n) ** 2 for n in sizes], None, None
+    before = [[t.clone() for t in ts] for ts in (theta, m, v, *((me, ve) if bits == 8 else ()))]
+    norm = float(torch.sqrt(sum((t.double() ** 2).sum() for t in grads)))
+    scale = clip / max(clip, norm) if clip else 1.0
+    state = torch.tensor([3, 0, 0], dtype=torch.int64, device="cuda")
+    plan = ops.AdamWPlan(theta, grads, m, v, 0.1, m_exp=me, v_exp=ve, params_lp=lp)
+    ops.adamw_step(plan, state, 1e-3, 0.9, 0.999, 1e-7, clip_norm=clip, seed=21)
+    assert int(state[0]) == 4
+    alpha = 1e-3 * np.sqrt(1 - 0.999 ** 4) / (1 - 0.9 ** 4)
+    slack = 10 * U if clip else 0.0  # of the norm, as in the test of the clip
+    first = np.cumsum([0] + blocks)
+    for i, n in enumerate(sizes):
+        assert torch.equal(lp[i], theta[i].to(torch.bfloat16))
+        for b in sorted({0, blocks[i] - 1, *rng.integers(0, blocks[i], 60).tolist()}):
+            s = slice(256 * b, min(256 * b + 256, n))
+            pick = lambda t: t[s].cpu().numpy()  # noqa: E731
+            if bits == 8:
+                old = [Moments8.decode(pick(before[1 + j][i]), before[3 + j][i][b:b + 1].cpu().numpy(), 4 + j) for j in (0, 1)]
+            else:
+                old = [pick(before[1][i]), pick(before[2][i])]
+            g64 = pick(grads[i]).astype(np.float64) * scale
+            th, mw, vw = np_ops.adamw_step(pick(before[0][i]), g64, old[0].astype(np.float64), old[1].astype(np.float64), 3, 1e-3, 0.1)
+            e_g = np.abs(g64) * (U + slack)
+            e_m = 4 * U * (np.abs(0.9 * old[0]) + np.abs(0.1 * g64)) + 0.1 * e_g
+            e_v = 5 * U * vw + 2e-3 * np.abs(g64) * e_g
+            step = alpha * mw / (np.sqrt(vw) + 1e-7)
+            e_step = 8 * U * np.abs(step) + alpha * e_m / (np.sqrt(vw) + 1e-7) + np.abs(step) * e_v / np.maximum(2 * vw, 1e-300)
+            assert (np.abs(pick(theta[i]) - th) <= e_step + 4 * U * (np.abs(pick(before[0][i])) + np.abs(th))).all(), (i, b)
+            if bits == 32:
+                assert (np.abs(pick(m[i]) - mw) <= e_m).all() and (np.abs(pick(v[i]) - vw) <= e_v).all(), (i, b)
+            elif not clip:
+                gs = pick(grads[i])
+                rnd = Moments8.random_bits(s.stop - s.start, int(first[i]) + b, 3, 21)
+                for val, r, width, ct, et in ((F(0.9) * old[0] + F(1 - 0.9) * gs, rnd[0], 4, m[i], me[i]),
+                                              (F(0.999) * old[1] + F(1 - 0.999) * (gs * gs), rnd[1], 5, v[i], ve[i])):
+                    code, exp = Moments8.encode(val, r, width)
+                    assert int(et[b]) == exp[0] and np.array_equal(pick(ct), code), (i, b, width)
+    if bits == 8:  # decoding of the same sizes
+        for i, n in enumerate(sizes):
+            out = torch.empty(n, device="cuda")
+            for second, ct, et in ((False, m[i], me[i]), (True, v[i], ve[i])):
+                ops.adamw_decode(ct, et, out, second)
+                for b in sorted({0, blocks[i] - 1, *rng.integers(0, blocks[i], 20).tolist()}):
+                    s = slice(256 * b, min(256 * b + 256, n))
+                    want = Moments8.decode(ct[s].cpu().numpy(), et[b:b + 1].cpu().numpy(), 5 if second else 4)
+                    assert np.array_equal(out[s].cpu().numpy(), want)
+
+
+def test_decoding_more_than_the_caches_hold():
+    from spectrum_vae_amd import ops
+    n = 70_000_003
+    g = torch.Generator(device="cuda").manual_seed(1)
+    codes = torch.randint(0, 256, (n,), dtype=torch.uint8, device="cuda", generator=g)
+    exps = torch.randint(0, 256, (-(-n // 256),), dtype=torch.uint8, device="cuda", generator=g)
+    whole = torch.full((n + 9,), 7.0, device="cuda")
+    for second in (False, True):
+        for off in (0, 1):  # with and without 16-byte accesses
+            out = whole[off:off + n]
+            ops.adamw_decode(codes, exps, out, second)
+            for b in (0, 1, 1000, 136_718, exps.numel() - 1):
+                s = slice(256 * b, min(256 * b + 256, n))
+                want = Moments8.decode(codes[s].cpu().numpy(), exps[b:b + 1].cpu().numpy(), 5 if second else 4)
+                assert np.array_equal(out[s].cpu().numpy(), want, equal_nan=True)
+            assert (whole[n + 1:] == 7).all()
+
+
 # ------------------------------------------------------------------------------------------------ in models
 def _model(optimizer, dtype="float32"):
     from spectrum_vae_amd import losses, mixed_precision

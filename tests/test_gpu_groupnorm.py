@@ -287,3 +287,110 @@ def test_gradients_against_differences():
     f = lambda t: (np_ops.group_norm(k.x + t * direction, k.gamma, k.beta, 4, EPS, "tanh")[0] * k.dy).sum()  # noqa: E731
     curve = abs((f(h) - f(-h)) / (2 * h) - (f(1e-5) - f(-1e-5)) / 2e-5)
     assert abs(num - ana) <= 2 * curve + 2 * 6e-7 * np.abs(k.dy).sum() / (2 * h) / np.sqrt(960) + 1e-4
+
+
+# Rows and channels that lie on both sides of every length at which the work is laid out differently: samples kept on the chip from
+# 64 rows of one line to some thousands, more samples than one and more slabs than one, groups that end inside a slab, samples too
+# long to keep with few and with many parts.
+LAYOUTS = [
+    ((33, 16, 64), 8), ((33, 64, 64), 8), ((33, 65, 64), 8), ((33, 129, 64), 8), ((33, 257, 64), 8), ((33, 1024, 64), 8),
+    ((17, 1025, 64), 8), ((33, 1100, 64), 4), ((33, 2049, 32), 4), ((33, 257, 40), 8), ((70, 520, 40), 8), ((33, 1030, 40), 8),
+    ((70, 2050, 20), 4), ((150, 12, 256), 16), ((151, 50, 96), 12), ((9, 100, 512), 4), ((3, 300, 1500), 12), ((2, 300, 4000), 32),
+    ((2, 5000, 36), 9), ((4, 8200, 27), 3), ((20, 4100, 6), 2), ((1, 70_000, 8), 8), ((300, 1, 48), 3), ((2100, 3, 6), 3),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,groups", LAYOUTS)
+def test_every_layout(shape, groups, dtype):
+    k = Case(shape, groups, "tanh", dtype, seed=17)
+    k.check_forward(*k.forward())
+    k.check_backward(*k.backward())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,groups", [((5, 8, 8, 64), 8), ((2, 96, 80, 36), 4), ((3, 300, 1500), 12)])
+def test_in_place(shape, groups, dtype):
+    """y may be x, and dx may be dy or x: every element is read before it is written, by the thread that writes it."""
+    k = Case(shape, groups, "elu", dtype, seed=1)
+    y, mean, rstd = k.forward()
+    x = k.xt.clone()
+    got = k.forward(x, x)
+    assert all(torch.equal(a, b) for a, b in zip(got, (y, mean, rstd)))
+    want = k.backward()
+    dy, x = k.dyt.clone(), k.xt.clone()
+    for got in (k.backward(None, dy, dy), k.backward(x, None, x)):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def _reference_pieces(x, dy, gamma, beta, mean, rstd, act_slope, act):
+    """z, dz, xhat in float64 of rows [r, C] of one sample."""
+    c = x.shape[-1]
+    rep = lambda t: t.double().repeat_interleave(c // t.numel())  # noqa: E731
+    xhat = (x.double() - rep(mean)) * rep(rstd)
+    z = xhat * gamma.double() + beta.double()
+    return xhat, act(z), (dy.double() * act_slope(z) if dy is not None else None)
+
+
+@pytest.mark.parametrize("shape,groups", [((1, 68_000_000, 32), 4), ((600_000, 64, 64), 8)])
+def test_more_than_2_to_the_31_elements(shape, groups):
+    """One sample, and many, of more elements than 31 bits count.  Chains of up to L = 68e6 / 2048 / 64 = 519 rows a thread: a mean
+    is off by at most L u of the mean magnitude (below 2 at unit spread), likewise the backward means and the channel sums."""
+    from spectrum_vae_amd import ops
+    n, s, c = shape
+    L, half = 520, 2.0 ** -8
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x, dy = (torch.empty(shape, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    for t in (x, dy):
+        for part in t.view(-1).split(1 << 28):
+            part.normal_(0.25, 1.0, generator=g)
+    gamma, beta = 1 + 0.1 * torch.randn(c, device="cuda", generator=g), 0.1 * torch.randn(c, device="cuda", generator=g)
+    y, mean, rstd = torch.empty_like(x), torch.empty(n, groups, device="cuda"), torch.empty(n, groups, device="cuda")
+    ws = torch.empty(ops.groupnorm_workspace(n, s, c, groups), dtype=torch.uint8, device="cuda")
+    ops.groupnorm_act_fwd(x, gamma, beta, y, mean, rstd, groups, EPS, "tanh", 0.0, ws)
+    slope = lambda z: 1 - torch.tanh(z) ** 2  # noqa: E731
+    d = c // groups
+    per = 1 << 20
+    looked = [0] if n == 1 else [0, 1, n // 2, n - 1]
+    sums = {}
+    for i in looked:
+        tot, sq = torch.zeros(groups, device="cuda", dtype=torch.float64), torch.zeros(groups, device="cuda", dtype=torch.float64)
+        for a in range(0, s, per):
+            q = x[i, a:a + per].double().view(-1, groups, d)
+            tot += q.sum(dim=(0, 2))
+            sq += (q * q).sum(dim=(0, 2))
+        mu = tot / (s * d)
+        rs = (sq / (s * d) - mu * mu + EPS).rsqrt()
+        assert ((mean[i].double() - mu).abs() <= 2 * L * U).all()
+        assert ((rstd[i].double() / rs - 1).abs() <= 2 * L * U).all()
+        sums[i] = (mu, rs)
+        for a in (0, s // 2, s - 7):
+            _, want, _ = _reference_pieces(x[i, a:a + 7], None, gamma, beta, mu, rs, slope, torch.tanh)
+            assert ((y[i, a:a + 7].double() - want).abs() <= half * want.abs() + 8 * L * U).all()
+    dx, dgamma, dbeta = y, torch.empty(c, device="cuda"), torch.empty(c, device="cuda")
+    ops.groupnorm_act_bwd(x, dy, gamma, beta, mean, rstd, dx, dgamma, dbeta, False, groups, "tanh", 0.0, ws)
+    for i in looked:
+        c1, c2 = torch.zeros(groups, device="cuda", dtype=torch.float64), torch.zeros(groups, device="cuda", dtype=torch.float64)
+        for a in range(0, s, per):
+            xhat, _, dz = _reference_pieces(x[i, a:a + per], dy[i, a:a + per], gamma, beta, mean[i], rstd[i], slope, torch.tanh)
+            gz = (dz * gamma.double()).view(-1, groups, d)
+            c1 += gz.sum(dim=(0, 2))
+            c2 += (gz * xhat.view(-1, groups, d)).sum(dim=(0, 2))
+        c1, c2 = (t.repeat_interleave(d) / (s * d) for t in (c1, c2))
+        for a in (0, s // 2, s - 7):
+            xhat, _, dz = _reference_pieces(x[i, a:a + 7], dy[i, a:a + 7], gamma, beta, mean[i], rstd[i], slope, torch.tanh)
+            want = rstd[i].double().repeat_interleave(d) * (dz * gamma.double() - c1 - xhat * c2)
+            assert ((dx[i, a:a + 7].double() - want).abs() <= half * want.abs() + 8 * L * U * (1 + xhat.abs() + dz.abs())).all()
+    dg, db, mag = (torch.zeros(c, device="cuda", dtype=torch.float64) for _ in range(3))
+    rows, step = x.view(-1, c), per // s * s if n > 1 else per
+    for a in range(0, n * s, step):
+        q = slice(a, a + step)
+        st = (mean, rstd) if n == 1 else (mean[a // s:(a + step) // s], rstd[a // s:(a + step) // s])
+        at = [t.double().repeat_interleave(d, dim=1).repeat_interleave(1 if n == 1 else s, dim=0) for t in st]
+        xhat = (rows[q].double() - at[0]) * at[1]
+        dz = dy.view(-1, c)[q].double() * slope(xhat * gamma.double() + beta.double())
+        dg += (dz * xhat).sum(dim=0)
+        db += dz.sum(dim=0)
+        mag += (dz.abs() * (1 + xhat.abs())).sum(dim=0)
+    # up to L terms in a chain, and 10 u of each term's own (statistics, activation, products)
+    assert ((dgamma.double() - dg).abs() <= (L + 10) * U * mag).all() and ((dbeta.double() - db).abs() <= (L + 10) * U * mag).all()

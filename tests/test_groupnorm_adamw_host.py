@@ -142,6 +142,31 @@ def test_adamw_arguments():
         opt.apply_model(None, slabs=[1])
 
 
+def test_epsilons_out_of_range():
+    from spectrum_vae_amd import _lib
+    from spectrum_vae_amd.optimizers import AdamW
+    with pytest.raises(ValueError, match="epsilon"):
+        AdamW(epsilon=1e-13)
+    p = 4096  # never read: the calls are refused before a launch
+    for eps in (0.0, 1e-13, float("nan")):
+        assert _lib.lib.sv_adamw_step(p, 1, 32, p, 1e-3, 0.9, 0.999, eps, 10, 0.9, 1, 1.0, 0.0, 0, 0, p, 1 << 20, None) == -1
+        assert "epsilon" in _lib.last_error()
+    for eps in (-1e-3, float("nan")):
+        assert _lib.lib.sv_groupnorm_act_fwd(p, p, p, p, p, p, 2, 4, 8, 2, eps, 0, 0.2, p, 1 << 20, 0, None) == -1
+        assert "epsilon" in _lib.last_error()
+
+
+def test_more_workgroups_than_a_launch_takes():
+    from spectrum_vae_amd import _lib
+    p = 4096  # never read
+    for n, s, c, g in ((1 << 24, 1, 32, 4), (1 << 23, 300, 130, 2)):
+        need = _lib.lib.sv_groupnorm_workspace_bytes(n, s, c, g)
+        assert _lib.lib.sv_groupnorm_act_fwd(p, p, p, p, p, p, n, s, c, g, 1e-3, 0, 0.2, p, need, 0, None) == -1
+        assert "too many" in _lib.last_error()
+        assert _lib.lib.sv_groupnorm_act_bwd(p, p, p, p, p, p, p, p, p, 0, n, s, c, g, 0, 0.2, p, need, 0, None) == -1
+        assert "too many" in _lib.last_error()
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 def test_groupnorm_refusals():
     from spectrum_vae_amd import _lib, ops
