@@ -849,7 +849,9 @@ __global__ __launch_bounds__(kStreamThreads, BWD && V == 8 ? 4 : 8) void gn_appl
                     v[e] = act_apply(z, decltype(act)::value, a.alpha);
                 }
             }
-            piece_at<Piece<T, V>>(out, col + at * pitch) = put<T, V>(v);
+            // nontemporal: the results then leave the caches' room to what is still to be read again (2 images of 512x512x128 bf16
+            // forward 96 -> 85 us, f32 backward 255 -> 236; no size gets slower)
+            __builtin_nontemporal_store(put<T, V>(v), &piece_at<Piece<T, V>>(out, col + at * pitch));
         };
         int at = r;
         for (; at + (U - 1) * rpb < rows; at += U * rpb) {
