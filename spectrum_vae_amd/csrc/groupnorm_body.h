@@ -930,19 +930,21 @@ constexpr bool held_compiled(bool bwd, int size, int piece, int K, int NT, bool 
 
 // Held where a slab of whole groups fits the registers of a workgroup, in the first form of the list that does.
 GnPlan gn_plan(int64_t N, int64_t S, int C, int G, int size, uintptr_t bits, bool bwd) {
-    // Bytes of a slab's row, pieces a thread, threads.  Rows of a cache line (128 bytes) first, in workgroups of 256, several a CU,
-    // whose phases overlap.  A sample of more rows in 64-byte rows with 512 threads before 128-byte ones with 1024, of which a CU
-    // holds one (512 samples of 32x32x64 bf16 forward 40 against 47 us, f32 backward 92 against 104) - but for the f32 forward
-    // pass of whole groups, of which it holds two (1024 samples of 32x32x64 111 against 125 us).  Below 64 bytes a
-    // row the streamed form is faster, and where fewer than 64 workgroups would hold 4096 pieces and more each: it spreads them (16
-    // samples of 40x40x48 bf16 backward 12.8 against 17.9 us, 8 of 64x64x64 forward 12.9 against 18.8; from 128 workgroups on
-    // the held form wins, 32 samples of 32x32x64 f32 forward 11.2 against 12.5).
+    // Bytes of a slab's row, pieces a thread, threads.  Rows of a cache line (128 bytes) first, in workgroups of 256 and 512, several
+    // a CU, whose phases overlap (1024 samples of 20x20x64 f32 with 512 threads forward 43 us and backward 64; with two
+    // workgroups of 1024 threads a CU forward 57, in 64-byte rows backward 78).  A sample of more rows in 64-byte rows with 512
+    // threads before 128-byte ones with 1024, of which a CU holds one (512 samples of 32x32x64 bf16 forward 32 against 41 us, 1024 of
+    // 30x30x96 94 against 133; backward 59 against 57, 139 against 183) - but for the f32 forward pass of whole groups, of which it
+    // holds two (1024 samples of 32x32x64 111 against 125 us).  Below 64 bytes a row the streamed form is faster, and where fewer
+    // than 64 workgroups would hold 4096 pieces and more each: it spreads them (16 samples of 40x40x48 bf16 backward 12.8 against
+    // 17.9 us, 8 of 64x64x64 forward 12.9 against 18.8; from 128 workgroups on the held form wins, 32 samples of 32x32x64 f32
+    // forward 11.2 against 12.5).
     struct Form {
         int row, K, NT;
         bool two;
     };
-    static const Form forms[] = {{128, 2, 256, false}, {128, 4, 256, false}, {128, 8, 256, false}, {128, 8, 1024, true},
-                                 {64, 8, 512, false},  {128, 8, 512, false}, {128, 8, 1024, false}, {64, 8, 1024, false},
+    static const Form forms[] = {{128, 2, 256, false}, {128, 4, 256, false}, {128, 8, 256, false}, {128, 8, 512, false}, {128, 8, 1024, true},
+                                 {64, 8, 512, false},  {128, 8, 1024, false}, {64, 8, 1024, false},
                                  {128, 16, 1024, false}, {64, 16, 1024, false}};
     GnPlan q{};
     q.V = piece_of(C, size, bits);
