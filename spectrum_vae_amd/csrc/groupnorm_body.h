@@ -812,7 +812,8 @@ __global__ __launch_bounds__(kStreamThreads, BWD && V == 8 ? 4 : 8) void gn_appl
     const int first = slab * a.CB, P = a.P, rpb = NT / P;
     const int last = first + a.CB < a.C ? first + a.CB : a.C;
     const int g0 = first / a.D, g1 = (last - 1) / a.D + 1, gs = g1 - g0;
-    const int lanes = lanes_for(a.groups != nullptr ? a.chunks : a.D);
+    int lanes = lanes_for(a.groups != nullptr ? a.chunks : a.D);
+    while (lanes > 1 && lanes * gs > NT) lanes >>= 1;  // all groups at once: a round of them costs about 1 us
     for (int g = g0 + threadIdx.x / lanes; g < g1; g += NT / lanes) {
         float u, v;
         group_values<BWD>(a, n, g, threadIdx.x % lanes, lanes, u, v);
