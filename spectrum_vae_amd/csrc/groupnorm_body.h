@@ -8,7 +8,17 @@
 //
 // Two forms.  HELD: a workgroup owns all rows of one sample for a slab of channels (whole groups) and keeps them in registers
 // between the statistics and the result, so a tensor crosses the memory bus once.  STREAMED, where a slab does not fit:
-// sums per chunk of rows, a fold over the chunks, and a second pass over the tensors.
+// sums per chunk of rows, a fold over the chunks (a launch, or the start of the second pass), and a second pass over the tensors.
+//
+// What bounds it: the memory, 8 flops a byte at most.  A copy of 512 MB runs at 5.3 TB/s here, and a launch that does next to nothing
+// takes 3.5 us.  Measured, with alternating tensors:
+//   held      forward   1024 x 32x32x64 f32     537 MB moved   100 us   5.4 TB/s
+//             forward   512 x 32x32x64 bf16     134 MB          32 us   4.2
+//             backward  1024 x 16x16x256 bf16   403 MB          83 us   4.8   (6 us of it gn_param_fold_k)
+//             forward   1 x 8x8x64 f32                         3.7 us
+//             backward  64 x 8x8x128 f32          6 MB         7.2 us   two launches
+//   streamed  forward   2 x 512x512x128 bf16    268 MB          84 us   403 MB with the second reading: 4.8 TB/s
+//             backward  4 x 256x256x64 f32      201 MB          64 us   336 MB with the second reading: 5.2 TB/s
 #pragma once
 #include <type_traits>
 
@@ -937,9 +947,9 @@ GnPlan gn_plan(int64_t N, int64_t S, int C, int G, int size, uintptr_t bits, boo
     // threads before 128-byte ones with 1024, of which a CU holds one (512 samples of 32x32x64 bf16 forward 32 against 41 us, 1024 of
     // 30x30x96 94 against 133; backward 59 against 57, 139 against 183) - but for the f32 forward pass of whole groups, of which it
     // holds two (1024 samples of 32x32x64 111 against 125 us).  Below 64 bytes a row the streamed form is faster, and where fewer
-    // than 64 workgroups would hold 4096 pieces and more each: it spreads them (16 samples of 40x40x48 bf16 backward 12.8 against
-    // 17.9 us, 8 of 64x64x64 forward 12.9 against 18.8; from 128 workgroups on the held form wins, 32 samples of 32x32x64 f32
-    // forward 11.2 against 12.5).
+    // than 48 workgroups would hold 4096 pieces and more each: it spreads them (16 samples of 40x40x48 bf16, 32 workgroups, backward
+    // 12.8 against 17.9 us, 8 of 64x64x64 forward 12.9 against 18.8; with 62 workgroups, 31 samples of 239x5x64 bf16, forward 13.3
+    // against 11.6).
     struct Form {
         int row, K, NT;
         bool two;
@@ -963,7 +973,7 @@ GnPlan gn_plan(int64_t N, int64_t S, int C, int G, int size, uintptr_t bits, boo
         const bool groups = log2_of(D) >= 0 && D >= q.V && P == 1 << log_q && P <= 64 && piece >= 8;
         if (cb > kHeldMaxC || 1 << log_q > f.NT || f.K * piece > most || S > (int64_t)f.K * f.NT >> log_q ||
             f.NT / (log_q < 6 ? 64 : 1 << log_q) * cb > kHeldSlots || (f.two && !(groups && size == 4 && !bwd)) ||
-            !held_compiled(bwd, size, piece, f.K, f.NT, groups) || (f.K * f.NT >= 4096 && N * ceil_div(C, cb) < 64))
+            !held_compiled(bwd, size, piece, f.K, f.NT, groups) || (f.K * f.NT >= 4096 && N * ceil_div(C, cb) < 48))
             continue;
         q.K = f.K;
         q.NT = f.NT;
@@ -1111,10 +1121,12 @@ int launch(const char* who, GnArgs& a, void* workspace, hipStream_t st) {
                                a.N, a.C, a.accumulate);
     } else {
         a.part = a.folded + a.N * 2 * a.C;
-        // Few chunks and whole groups in a slab: the second pass joins the groups' values itself, which saves a launch (32 samples of
-        // 128x128x32 bf16 forward 28.2 -> 26.9 us, backward 38.1 -> 37.1; at two samples of 512x512 and 1024 chunks each 29.7 -> 38.3).
-        // Backward, its first workgroups also add the channels' sums of all chunks.
-        if (q.slabs == 1 && q.chunks <= 64 && (!BWD || a.N * q.chunks <= 2048)) a.groups = a.part + a.N * q.chunks * 2 * a.C;
+        // Whole groups in a slab and few chunks: the second pass joins the groups' values itself, which saves a launch (32 samples of
+        // 128x128x32 bf16 forward 28.2 -> 26.9 us, backward 38.1 -> 37.1; one of 18x67x10 f32 9.7 -> 9.0).  All of its workgroups read
+        // all of a sample's values: more than 10 MB in all cost more than the launch (two samples of 512x512x32 bf16, 1024 chunks
+        // each, 29.7 -> 38.3).  Backward, its first workgroups also add the channels' sums of all chunks.
+        if (q.slabs == 1 && a.N * q.chunks * q.chunks * a.G <= 5 << 18 && (!BWD || a.N * q.chunks <= 2048))
+            a.groups = a.part + a.N * q.chunks * 2 * a.C;
         launch_streamed<T, BWD>(a, q, st);
     }
     return check_launch(who);
