@@ -13,6 +13,12 @@
 // changes by 0.1 % a step, and rounding to nearest at 3 bits (steps of 12 %) would never move it.  A positive second moment never
 // becomes 0 (the step would divide by eps alone).  All arithmetic is in 32 bits with every rounding spelled out; theta's step
 // uses the moments before they are rounded.
+//
+// What bounds it: the memory.  A weight moves 28 bytes with 32-bit moments (theta, m, v both ways, the gradient), 16.02 with 8-bit
+// ones, for about 16 flops.  Measured where a copy runs at 5.3 TB/s and a launch that does next to nothing takes 3.5 us:
+//   101 M weights   adamw_k<32>  482 us  5.9 TB/s;  grad_norm_k  68 us  5.9;  adamw_k<8>  304 us  5.3;  adamw_decode_k  94 us  5.4
+//   0.8 M weights   adamw_k<8> with a bf16 copy  7.8 us;  adamw_decode_k  2.8 us
+//   12 thousand weights in 12 tensors   adamw_k<32>  4.4 us
 #include <algorithm>
 #include <new>
 #include <vector>

@@ -357,6 +357,51 @@ def test_decoding_more_than_the_caches_hold():
             assert (whole[n + 1:] == 7).all()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_two_plans_at_once_and_two_recordings_of_each(bits):
+    """Plans of different tensors stepped on two streams at once, eagerly and by graphs recorded twice from one plan: the bits of
+    steps one after the other."""
+    from spectrum_vae_amd import ops
+
+    def make(seed):
+        t = Tensors([300, 70_001, 8193, 4096 * 70], bits, seed=seed)
+        return t, t.plan(), torch.zeros(3, dtype=torch.int64, device="cuda")
+
+    def step(plan, state):
+        ops.adamw_step(plan, state, 1e-3, 0.9, 0.999, 1e-7, clip_norm=0.2, seed=3)
+
+    alone = [make(s) for s in (1, 2)]
+    for _, plan, state in alone:
+        for _ in range(5):
+            step(plan, state)
+    torch.cuda.synchronize()
+    both = [make(s) for s in (1, 2)]
+    graphs = []
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for (_, plan, state), st in zip(both, streams):  # two eager steps, then three replays of two recordings
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            step(plan, state)
+            step(plan, state)
+    torch.cuda.synchronize()
+    for _, plan, state in both:
+        pair = []
+        for _ in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                step(plan, state)
+            pair.append(g)
+        graphs.append(pair)
+    for k in (0, 1, 0):
+        for pair, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                pair[k].replay()
+    torch.cuda.synchronize()
+    for (a, _, sa), (b, _, sb) in zip(alone, both):
+        assert int(sa[0]) == int(sb[0]) == 5
+        assert all(torch.equal(x, y) for x, y in zip(a.theta_t + a.m_t + a.v_t + a.lp_t, b.theta_t + b.m_t + b.v_t + b.lp_t))
+
+
 # ------------------------------------------------------------------------------------------------ in models
 def _model(optimizer, dtype="float32"):
     from spectrum_vae_amd import losses, mixed_precision

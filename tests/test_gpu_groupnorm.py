@@ -394,3 +394,95 @@ def test_more_than_2_to_the_31_elements(shape, groups):
         mag += (dz.abs() * (1 + xhat.abs())).sum(dim=0)
     # up to L terms in a chain, and 10 u of each term's own (statistics, activation, products)
     assert ((dgamma.double() - dg).abs() <= (L + 10) * U * mag).all() and ((dbeta.double() - db).abs() <= (L + 10) * U * mag).all()
+
+
+def test_two_calls_at_once_and_two_graphs_with_one_workspace():
+    """Calls on two streams with workspaces of their own do not disturb each other; two recorded graphs that share a workspace
+    give the eager bits in any order of replays, with other work in between."""
+    from spectrum_vae_amd import ops
+    a, b = Case((3, 120, 100, 48), 6, "elu", torch.bfloat16), Case((4, 64, 70, 20), 4, "tanh", torch.float32)
+    want = [[t.clone() for t in (*k.forward(), *k.backward())] for k in (a, b)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        got = []
+        for st, k in zip(streams, (a, b)):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                got.append((*k.forward(), *k.backward()))
+        for st in streams:
+            torch.cuda.current_stream().wait_stream(st)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for g, w in zip(got, want) for x, y in zip(g, w))
+    nbytes = max(ops.groupnorm_workspace(k.shape[0], k.shape[1] * k.shape[2], k.shape[3], k.groups) for k in (a, b))
+    ws = torch.full((nbytes,), 255, dtype=torch.uint8, device="cuda")
+    graphs, outs = [], []
+    for k in (a, b):
+        y, mean, rstd = torch.empty_like(k.xt), *(torch.empty(k.shape[0], k.groups, device="cuda") for _ in range(2))
+        dx, dg, db = torch.empty_like(k.xt), *(torch.empty(k.shape[-1], device="cuda") for _ in range(2))
+
+        def run():
+            ops.groupnorm_act_fwd(k.xt, k.gt, k.bt, y, mean, rstd, k.groups, EPS, k.act, 0.2, ws)
+            ops.groupnorm_act_bwd(k.xt, k.dyt, k.gt, k.bt, k.mean, k.rstd, dx, dg, db, False, k.groups, k.act, 0.2, ws)
+
+        run()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run()
+        graphs.append(graph)
+        outs.append((y, mean, rstd, dx, dg, db))
+    for order in ((0, 1), (1, 0), (0, 0), (1, 1)):
+        for i in order:
+            for t in outs[i]:
+                t.fill_(7)
+            graphs[i].replay()
+            torch.zeros(1000, device="cuda").add_(1)
+        torch.cuda.synchronize()
+        for i in set(order):
+            assert all(torch.equal(x, y) for x, y in zip(outs[i], want[i]))
+
+
+def test_strided_tensors_and_other_types_are_refused():
+    from spectrum_vae_amd import ops
+    k = Case((2, 4, 4, 8), 2, None, torch.float32)
+    y, st = torch.empty_like(k.xt), torch.empty(2, 2, device="cuda")
+    call = lambda x, y, ws=None: ops.groupnorm_act_fwd(x, k.gt, k.bt, y, st, st.clone(), 2, EPS, None, 0.0, k.ws() if ws is None else ws)  # noqa: E731
+    for bad in (k.xt.transpose(1, 2), k.xt.half(), k.xt.double()):
+        with pytest.raises((TypeError, ValueError)):
+            call(bad, y)
+    with pytest.raises((TypeError, ValueError)):
+        call(k.xt, y.to(torch.bfloat16))
+    with pytest.raises(ValueError, match="one device"):
+        ops.groupnorm_act_fwd(k.xt, k.gt.cpu(), k.bt, y, st, st.clone(), 2, EPS, None, 0.0, k.ws())
+    from spectrum_vae_amd import _lib
+    with pytest.raises(_lib.SpectrumHipError, match="workspace"):
+        call(k.xt, y, k.ws()[:16])
+
+
+def test_a_view_of_half_a_call_goes_back_as_a_call_of_its_own():
+    """The generated half of a discriminator's [real; generated] call: the gradient through the view is that of a call on those
+    samples alone, and inference gives what the training call gave."""
+    from spectrum_vae_amd import unet
+    rng = np.random.default_rng(6)
+    disc = unet.Discriminator(normalization="group")
+    disc.build_graph((1, 32, 32, 4))
+    disc._materialize(torch.device("cuda", 0))
+    both = torch.from_numpy(rng.standard_normal((6, 32, 32, 4)).astype(np.float32)).cuda()
+    z = disc.forward_raw(both, True, bn_groups=2).clone()
+    dz = torch.from_numpy(rng.standard_normal(tuple(z[3:].shape)).astype(np.float32)).cuda()
+    view = disc._calls[0].group_view(1)
+    view.param_grads = False
+    disc.zero_grad_raw()
+    through = disc.backward(view, dz, need_dx=True).clone()
+    assert not disc._grads.any()
+    alone = unet.Discriminator(normalization="group")
+    alone.build_graph((1, 32, 32, 4))
+    alone._materialize(torch.device("cuda", 0))
+    alone._params.copy_(disc._params)
+    z_alone = alone.forward_raw(both[3:].contiguous(), True).clone()
+    # layers of other extents may sum in another order
+    assert torch.allclose(z_alone, z[3:], rtol=1e-4, atol=1e-5)
+    dx = alone.backward(alone._calls[0], dz.clone(), need_dx=True)
+    assert float((dx - through).norm() / through.norm()) <= 1e-4
+    one = disc.predict(both[4:5].cpu().numpy(), batch_size=1)
+    assert np.allclose(one.reshape(-1), z[4].cpu().numpy().reshape(-1), rtol=1e-4, atol=1e-5)
