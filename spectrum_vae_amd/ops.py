@@ -548,6 +548,16 @@ def _f32(t) -> Optional[int]:
     return t.data_ptr() if t.dtype is torch.float32 and t.is_contiguous() else _ptr(t)
 
 
+def _act_here(t, like, name: str) -> int:
+    """``_aptr`` of a tensor whose device ``_here`` has seen."""
+    return t.data_ptr() if t.dtype is like.dtype and t.is_contiguous() else _aptr(t, like, name)
+
+
+def _ws_here(ws):
+    """``_ws_args`` of a workspace whose device ``_here`` has seen."""
+    return (ws.data_ptr(), ws.numel()) if ws is not None and ws.dtype is torch.uint8 and ws.is_contiguous() else _ws_args(ws)
+
+
 def groupnorm_workspace(n: int, s: int, c: int, groups: int) -> int:
     """Scratch bytes of ``groupnorm_act_fwd`` / ``groupnorm_act_bwd`` on [n, s, c] activations (s: product of the spatial
     extents)."""
@@ -582,8 +592,9 @@ def groupnorm_act_fwd(x, gamma, beta, y, save_mean, save_rstd, groups: int, eps:
     if stream is None:
         with torch.cuda.device(x.device):
             return groupnorm_act_fwd(x, gamma, beta, y, save_mean, save_rstd, groups, eps, act, alpha, ws)
-    check(lib.sv_groupnorm_act_fwd(_aptr(x), _f32(gamma), _f32(beta), _aptr(y, x, "y"), _f32(save_mean), _f32(save_rstd), n, s,
-                                   c, groups, eps, ACT[act], alpha, *_ws_args(ws), _dt(x), stream), "sv_groupnorm_act_fwd")
+    check(lib.sv_groupnorm_act_fwd(_act_here(x, x, "x"), _f32(gamma), _f32(beta), _act_here(y, x, "y"), _f32(save_mean),
+                                   _f32(save_rstd), n, s, c, groups, eps, ACT[act], alpha, *_ws_here(ws), _dt(x), stream),
+          "sv_groupnorm_act_fwd")
 
 
 def groupnorm_act_bwd(x, dy, gamma, beta, save_mean, save_rstd, dx, dgamma, dbeta, accumulate: bool, groups: int, act,
@@ -599,9 +610,9 @@ def groupnorm_act_bwd(x, dy, gamma, beta, save_mean, save_rstd, dx, dgamma, dbet
     if stream is None:
         with torch.cuda.device(x.device):
             return groupnorm_act_bwd(x, dy, gamma, beta, save_mean, save_rstd, dx, dgamma, dbeta, accumulate, groups, act, alpha, ws)
-    check(lib.sv_groupnorm_act_bwd(_aptr(x), _aptr(dy, x, "dy"), _f32(gamma), _f32(beta), _f32(save_mean), _f32(save_rstd),
-                                   _aptr(dx, x, "dx"), _f32(dgamma), _f32(dbeta), int(accumulate), n, s, c, groups, ACT[act],
-                                   alpha, *_ws_args(ws), _dt(x), stream), "sv_groupnorm_act_bwd")
+    check(lib.sv_groupnorm_act_bwd(_act_here(x, x, "x"), _act_here(dy, x, "dy"), _f32(gamma), _f32(beta), _f32(save_mean),
+                                   _f32(save_rstd), _act_here(dx, x, "dx"), _f32(dgamma), _f32(dbeta), int(accumulate), n, s, c,
+                                   groups, ACT[act], alpha, *_ws_here(ws), _dt(x), stream), "sv_groupnorm_act_bwd")
 
 
 def concat_channels_fwd(a, b, y, rows, ca, cb):
