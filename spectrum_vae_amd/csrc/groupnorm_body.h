@@ -946,10 +946,11 @@ GnPlan gn_plan(int64_t N, int64_t S, int C, int G, int size, uintptr_t bits, boo
     // workgroups of 1024 threads a CU forward 57, in 64-byte rows backward 78).  A sample of more rows in 64-byte rows with 512
     // threads before 128-byte ones with 1024, of which a CU holds one (512 samples of 32x32x64 bf16 forward 32 against 41 us, 1024 of
     // 30x30x96 94 against 133; backward 59 against 57, 139 against 183) - but for the f32 forward pass of whole groups, of which it
-    // holds two (1024 samples of 32x32x64 111 against 125 us).  Below 64 bytes a row the streamed form is faster, and where fewer
-    // than 48 workgroups would hold 4096 pieces and more each: it spreads them (16 samples of 40x40x48 bf16, 32 workgroups, backward
-    // 12.8 against 17.9 us, 8 of 64x64x64 forward 12.9 against 18.8; with 62 workgroups, 31 samples of 239x5x64 bf16, forward 13.3
-    // against 11.6).
+    // holds two (1024 samples of 32x32x64 111 against 125 us).  Below 64 bytes a row the streamed form is faster, and where few
+    // workgroups would hold much each: it spreads them.  Fewer than 112 of 8192 pieces and more (50 samples of 40x40x48 bf16, 100
+    // workgroups, forward 16.1 against 17.5 us, backward 17.4 against 22.4; 31 of 239x5x64, 62 workgroups, 14.5 against 13.6 and
+    // 14.8 against 18.2), fewer than 48 of 4096 (8 of 32x32x64 f32, 32 workgroups, 8.9 against 9.6 and 9.5 against 11.1; with 100
+    // workgroups, 25 of 32x32x128 bf16, 16.8 against 12.3 and 17.0 against 17.8).
     struct Form {
         int row, K, NT;
         bool two;
@@ -973,7 +974,7 @@ GnPlan gn_plan(int64_t N, int64_t S, int C, int G, int size, uintptr_t bits, boo
         const bool groups = log2_of(D) >= 0 && D >= q.V && P == 1 << log_q && P <= 64 && piece >= 8;
         if (cb > kHeldMaxC || 1 << log_q > f.NT || f.K * piece > most || S > (int64_t)f.K * f.NT >> log_q ||
             f.NT / (log_q < 6 ? 64 : 1 << log_q) * cb > kHeldSlots || (f.two && !(groups && size == 4 && !bwd)) ||
-            !held_compiled(bwd, size, piece, f.K, f.NT, groups) || (f.K * f.NT >= 4096 && N * ceil_div(C, cb) < 48))
+            !held_compiled(bwd, size, piece, f.K, f.NT, groups) || N * ceil_div(C, cb) < (f.K * f.NT >= 8192 ? 112 : f.K * f.NT >= 4096 ? 48 : 0))
             continue;
         q.K = f.K;
         q.NT = f.NT;
