@@ -29,7 +29,7 @@ namespace {
 
 constexpr int kGnMaxC = 4096;
 constexpr int kHeldMaxC = 512;                // widest slab of the held form
-constexpr int kHeldSlots = 4096;              // most slots x channels of it (LDS: 32 KB, and at most 8 for the groups)
+constexpr int kHeldSlots = 4096;              // most slots x channels of it (LDS: 32 KB, and at most 16 for the groups)
 constexpr int kHeldFwd = 256, kHeldBwd = 128;  // bytes of a tensor that a thread holds, forward and (each of two) backward
 
 __device__ __forceinline__ float norm_xhat(float x, float mean, float rstd) {
