@@ -388,6 +388,7 @@ int sv_batchnorm_sync_bwd_apply(const void* x, const void* dy, const void* y_act
  *  - save_mean / save_rstd [N, groups], f32: what the backward call needs; both may be NULL (inference).
  *  - backward: dgamma / dbeta (+)= the sums over N and S, formed in a fixed order.  The activation's slope is recomputed
  *    from x; at 0 it is that of the negative side.
+ *  - a NaN in a group makes all that is computed from the group NaN, behind ReLU too.
  *  - tensors need no alignment beyond their elements'.  y may be x, and dx may be dy or x; otherwise outputs must not overlap
  *    inputs.
  *  workspace: sv_groupnorm_workspace_bytes, 16-byte aligned, for either direction. */

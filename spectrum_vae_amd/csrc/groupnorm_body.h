@@ -96,7 +96,12 @@ __device__ __forceinline__ void with_act(int act, F f) {
         default: f(std::integral_constant<int, SV_ACT_NONE>{}); break;
     }
 }
-// d act / d z from z; at 0 the slope of the negative side.
+// act(z).  NaN stays NaN behind every activation (act_apply's ReLU makes it 0, and one such input would turn the whole group into
+// clean zeros).
+__device__ __forceinline__ float act_value(float z, int act, float alpha) {
+    return act == SV_ACT_RELU ? (z <= 0.f ? 0.f : z) : act_apply(z, act, alpha);
+}
+// d act / d z from z; at 0 the slope of the negative side (also where z is NaN and the slope has two values: see keep_nan).
 __device__ __forceinline__ float act_slope(float z, int act, float alpha) {
     switch (act) {
         case SV_ACT_RELU: return z > 0.f ? 1.f : 0.f;
@@ -106,6 +111,12 @@ __device__ __forceinline__ float act_slope(float z, int act, float alpha) {
         case SV_ACT_SIGMOID: { const float y = __builtin_amdgcn_rcpf(1.f + __expf(-z)); return y * (1.f - y); }
         default: return 1.f;
     }
+}
+// A channel's sums of dz and dz xhat where z was NaN and the slope did not show it: xhat did, or gamma or beta is NaN.  (Once a
+// channel; a slope that is NaN for NaN is a comparison more an element, 1 to 2 % of the whole backward pass.)
+__device__ __forceinline__ void keep_nan(float& dz, float& dz_xhat, float gamma, float beta, int act) {
+    if (act != SV_ACT_RELU && act != SV_ACT_LRELU) return;
+    if (dz_xhat != dz_xhat || gamma != gamma || beta != beta) dz = dz_xhat = __uint_as_float(0x7fc00000u);
 }
 
 // ------------------------------------------------------------------------------------------------ sums across lanes
@@ -350,7 +361,7 @@ __global__ __launch_bounds__(NT, (GROUPS && K * V * sizeof(T) <= 128 && sizeof(T
                 float o[V];
 #pragma unroll
                 for (int e = 0; e < V; ++e)
-                    o[e] = act_apply(norm_z(norm_xhat(get<T, V>(buf[k], e), mu[e], rs[e]), ga[e], be[e]), decltype(act)::value, a.alpha);
+                    o[e] = act_value(norm_z(norm_xhat(get<T, V>(buf[k], e), mu[e], rs[e]), ga[e], be[e]), decltype(act)::value, a.alpha);
                 store_piece<FAR != 0>(piece_at<Q_>(y, at0 + k * step), put<T, V>(o));
             }
     });
@@ -405,6 +416,8 @@ __global__ __launch_bounds__(NT) void gn_bwd_held_k(GnArgs a) {
                     s1[e] = fmaf(dz, xh, s1[e]);
                 }
             }
+#pragma unroll
+        for (int e = 0; e < V; ++e) keep_nan(s0[e], s1[e], ga[e], be[e], decltype(act)::value);
     });
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -586,6 +599,9 @@ __global__ __launch_bounds__(kStreamThreads, BWD && V == 8 ? 4 : 8) void gn_sums
                 const Piece<T, V> bx = piece_at<Q_>(x, col + at * pitch);
                 row(bx, BWD ? piece_at<Q_>(dy, col + at * pitch) : bx, act);
             }
+            if (BWD)
+#pragma unroll
+                for (int e = 0; e < V; ++e) keep_nan(acc[0][e], acc[1][e], ga[e], be[e], decltype(act)::value);
         };
         if (BWD) with_act(a.act, all);
         else all(std::integral_constant<int, SV_ACT_NONE>{});
@@ -867,7 +883,7 @@ __global__ __launch_bounds__(kStreamThreads, BWD && V == 8 ? 4 : 8) void gn_appl
                     const float dz = get<T, V>(bg, e) * act_slope(z, decltype(act)::value, a.alpha);
                     v[e] = fmaf(dz, rs[e] * ga[e], fmaf(xh, k1[e], k0[e]));
                 } else {
-                    v[e] = act_apply(z, decltype(act)::value, a.alpha);
+                    v[e] = act_value(z, decltype(act)::value, a.alpha);
                 }
             }
             // nontemporal: the results then leave the caches' room to what is still to be read again (2 images of 512x512x128 bf16
