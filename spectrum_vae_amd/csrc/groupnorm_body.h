@@ -525,12 +525,15 @@ __global__ __launch_bounds__(NT) void gn_bwd_held_k(GnArgs a) {
 // Workgroup -> (sample, chunk of rows, slab of channels); 256 threads, P = CB / V <= 256 pieces a row, rows r, r + 256 / P, ...
 constexpr int kStreamThreads = 256;
 __host__ __device__ __forceinline__ bool lanes_share(int P) { return P <= 64 && (P & (P - 1)) == 0; }
-// Per chunk and channel.  Forward: mean and sum of squared deviations (about the chunk's first row, then moved to the mean).
-// Backward: sum dz, sum dz xhat.
+// Per chunk and channel.  Forward: mean and sum of squared deviations from it.  A thread sums about the mean of the first U rows it
+// takes, which an outlier among them moves by a U-th only; its mean and squares are then joined with the other ones' by counts, across
+// lanes, waves and chunks.  So a sum of squares is cut down by L / U of itself at most, L the thread's rows.  (About the chunk's
+// first row, should that be the outlier - a border, padding -, it is cut down by as much as the chunk has rows: 0.3 everywhere behind a
+// first row of 1e4, 30 M rows, left rstd off by 1.3 %.)  Backward: sum dz, sum dz xhat.
 // Eight workgroups a CU: 2048 of them are resident at once (with eight bf16 channels a thread, backward, half of them).
 template <typename T, int V, bool BWD>
 __global__ __launch_bounds__(kStreamThreads, BWD && V == 8 ? 4 : 8) void gn_sums_k(GnArgs a) {
-    extern __shared__ float sm[];  // [2][rows at a time, or waves][channels of a slab] | [3][channels]
+    extern __shared__ float sm[];  // [2][parts: rows at a time, or waves][channels of a slab] | [3][channels] | [parts]
     constexpr int NT = kStreamThreads, U = BWD ? 2 : V == 8 ? 4 : 8;  // pieces of each tensor in flight
     const int slab = (int)(blockIdx.x % a.slabs);
     const int64_t i = blockIdx.x / a.slabs, n = i / a.chunks, chunk = i % a.chunks;
@@ -545,6 +548,8 @@ __global__ __launch_bounds__(kStreamThreads, BWD && V == 8 ? 4 : 8) void gn_sums
     typedef const Piece<T, V> Q_;
     const T *x = (const T*)a.x + base, *dy = (const T*)a.dy + base;
     float acc[2][V], mu[V], rs[V], ga[V], be[V];
+    Piece<T, V> pivot;  // (forward) the chunk's first row: what means are distances from until the end
+    float seen = 0.f;   // (forward) rows in acc
 #pragma unroll
     for (int e = 0; e < V; ++e) acc[0][e] = acc[1][e] = 0.f;
     if (on) {
@@ -557,9 +562,9 @@ __global__ __launch_bounds__(kStreamThreads, BWD && V == 8 ? 4 : 8) void gn_sums
                 ga[e] = a.gamma[c0 + e];
                 be[e] = a.beta[c0 + e];
             }
+        } else {
+            pivot = piece_at<Q_>(x, col);
         }
-        Piece<T, V> pivot;
-        if (!BWD) pivot = piece_at<Q_>(x, col);
         const auto row = [&](const Piece<T, V>& bx, const Piece<T, V>& bg, auto act) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
@@ -575,30 +580,46 @@ __global__ __launch_bounds__(kStreamThreads, BWD && V == 8 ? 4 : 8) void gn_sums
                 }
             }
         };
-        const auto about = [&] {  // behind the first loads, not ahead of them: the first row is waited for with them
-            if (BWD) return;
-            forget(pivot);
+        // U rows of this thread, or what is left of them, with all loads ahead of all sums
+        const auto block = [&](int at, auto whole, auto act) {
+            const auto there = [&](int u) { return decltype(whole)::value || at + u * rpb < rows; };
+            Piece<T, V> bx[U], bg[U];
 #pragma unroll
-            for (int e = 0; e < V; ++e) mu[e] = get<T, V>(pivot, e);
-        };
-        const auto all = [&](auto act) {
-            int at = r;
-            for (; at + (U - 1) * rpb < rows; at += U * rpb) {
-                Piece<T, V> bx[U], bg[U];
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
+            for (int u = 0; u < U; ++u)
+                if (there(u)) {
                     bx[u] = piece_at<Q_>(x, col + (at + u * rpb) * pitch);
                     if (BWD) bg[u] = piece_at<Q_>(dy, col + (at + u * rpb) * pitch);
                 }
-                about();
+            if constexpr (!BWD) {
+                float count = (float)U;
+                if (!decltype(whole)::value) {
+                    count = 0.f;
 #pragma unroll
-                for (int u = 0; u < U; ++u) row(bx[u], bg[u], act);
+                    for (int u = 0; u < U; ++u) count += there(u) ? 1.f : 0.f;
+                }
+                if (seen == 0.f) {  // the first ones
+                    const float inv = decltype(whole)::value ? 1.f / (float)U : __builtin_amdgcn_rcpf(count);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        float sum = 0.f;
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+                            if (there(u)) sum += get<T, V>(bx[u], e);
+                        mu[e] = sum * inv;
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; ++u) forget(bx[u]);
+                }
+                seen += count;
             }
-            about();
-            for (; at < rows; at += rpb) {
-                const Piece<T, V> bx = piece_at<Q_>(x, col + at * pitch);
-                row(bx, BWD ? piece_at<Q_>(dy, col + at * pitch) : bx, act);
-            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (there(u)) row(bx[u], bg[u], act);
+        };
+        const auto all = [&](auto act) {
+            int at = r;
+            for (; at + (U - 1) * rpb < rows; at += U * rpb) block(at, std::true_type{}, act);
+            if (at < rows) block(at, std::false_type{}, act);
             if (BWD)
 #pragma unroll
                 for (int e = 0; e < V; ++e) keep_nan(acc[0][e], acc[1][e], ga[e], be[e], decltype(act)::value);
@@ -606,15 +627,36 @@ __global__ __launch_bounds__(kStreamThreads, BWD && V == 8 ? 4 : 8) void gn_sums
         if (BWD) with_act(a.act, all);
         else all(std::integral_constant<int, SV_ACT_NONE>{});
     }
+    if (!BWD && on) {  // sums about mu -> mean and squares about it
+        const float inv = seen > 0.f ? __builtin_amdgcn_rcpf(seen) : 0.f;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float m = acc[0][e] * inv, first = get<T, V>(pivot, e);
+            acc[1][e] = fmaf(-acc[0][e], m, acc[1][e]);
+            acc[0][e] = seen > 0.f ? mu[e] - first + m : 0.f;
+            mu[e] = first;
+        }
+    }
     // rows together: across lanes where a wave holds whole rows (P a power of two), the rest through LDS
     const bool lanes = lanes_share(P);
     const int held = lanes ? NT / 64 : rpb, mine = lanes ? threadIdx.x >> 6 : r;
-    float *s1 = sm + held * CB, *first = s1 + held * CB;
-    if (lanes)
+    float *s1 = sm + held * CB, *first = s1 + held * CB, *count = first + 3 * CB;
+    if (lanes && BWD) {
 #pragma unroll
         for (int q = 0; q < 2; ++q)
 #pragma unroll
             for (int e = 0; e < V; ++e) acc[q][e] = sum_stride(acc[q][e], P);
+    } else if (lanes) {
+        const float all = sum_stride(seen, P), inv = all > 0.f ? __builtin_amdgcn_rcpf(all) : 0.f;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float m = sum_stride(seen * acc[0][e], P) * inv, d = acc[0][e] - m;
+            acc[1][e] = sum_stride(fmaf(seen * d, d, acc[1][e]), P);
+            acc[0][e] = m;
+        }
+        seen = all;
+    }
+    if (!BWD && p == 0 && r < rpb && (!lanes || (threadIdx.x & 63) == 0)) count[mine] = seen;
     if (on && (!lanes || (threadIdx.x & 63) < P))
 #pragma unroll
         for (int e = 0; e < V; ++e) {
@@ -624,19 +666,37 @@ __global__ __launch_bounds__(kStreamThreads, BWD && V == 8 ? 4 : 8) void gn_sums
         }
     __syncthreads();
     float* part = a.part + i * 2 * a.C + slab * CB;
-    for (int c = threadIdx.x; c < CB && slab * CB + c < a.C; c += NT) {
+    // few channels, many parts (forward): neighbouring lanes share a channel's parts, eight each (2 samples of 500x500x6 f32, whose three
+    // pieces a row leave 85 parts, 17.3 -> 15.3 us)
+    int shared = 1;
+    while (!BWD && shared < 8 && 2 * shared * CB <= NT && 16 * shared <= held) shared <<= 1;
+    const int sub = threadIdx.x & (shared - 1);
+    for (int c = threadIdx.x / shared; c < CB && slab * CB + c < a.C; c += NT / shared) {
         double u = 0.0, w = 0.0;
-        for (int k = 0; k < held; ++k) {
-            u += (double)sm[k * CB + c];
-            w += (double)s1[k * CB + c];
+        if (BWD) {
+            for (int k = 0; k < held; ++k) {
+                u += (double)sm[k * CB + c];
+                w += (double)s1[k * CB + c];
+            }
+        } else {  // parts' means and squares -> the chunk's: u = sum n mean, w = sum n mean^2 + squares
+            for (int k = sub; k < held; k += shared) {
+                const double x = (double)sm[k * CB + c], n0 = (double)count[k] * x;
+                u += n0;
+                w += fma(n0, x, (double)s1[k * CB + c]);
+            }
+            for (int o = shared >> 1; o > 0; o >>= 1) {
+                u += __shfl_xor(u, o, 64);
+                w += __shfl_xor(w, o, 64);
+            }
+            double inv = (double)__builtin_amdgcn_rcpf((float)rows);
+            inv = inv * fma(-(double)rows, inv, 2.0);  // 1 / rows to 2^-44
+            const double m = u * inv;
+            w = fma(-u, m, w);
+            w = w < 0.0 ? 0.0 : w;
+            u = (double)first[c] + m;
         }
-        float s = (float)u, q = (float)w;
-        if (!BWD) {  // sums about the first row -> mean, and squares about it
-            const float m = s / (float)rows;
-            q -= s * m;
-            q = q < 0.f ? 0.f : q;
-            s = first[c] + m;
-        }
+        const float s = (float)u, q = (float)w;
+        if (sub != 0) continue;
         if (BWD || a.groups == nullptr) {
             part[c] = s;
             part[a.C + c] = q;
@@ -1104,7 +1164,7 @@ template <typename T, bool BWD>
 void launch_streamed(const GnArgs& a, const GnPlan& q, hipStream_t st) {
     const int64_t main = a.N * q.chunks * q.slabs;
     const int held = lanes_share(q.P) ? kStreamThreads / 64 : kStreamThreads / q.P;
-    const size_t lds = (2 * (size_t)held + 3) * q.CB * sizeof(float);  // at most 40 KB
+    const size_t lds = ((2 * (size_t)held + 3) * q.CB + held) * sizeof(float);  // at most 41 KB
     const size_t lds_apply = 2 * ((size_t)q.CB / a.D + 2) * sizeof(float);
     with_piece<T>(q.V, [&](auto piece) {
         constexpr int V = decltype(piece)::value;
