@@ -139,6 +139,21 @@ class Adam:
                 "slots": {k: (m.cpu(), v.cpu()) for k, (m, v) in self._slots.items()}}
 
 
+def _apart(grads, written):
+    """The gradients, each that shares memory with another one or with a tensor of ``written`` as a copy of its own."""
+    spans = [(t.data_ptr(), 0, -1, t) for t in written] + [(g.data_ptr(), 1, i, g) for i, g in enumerate(grads)]
+    spans = sorted((s for s in spans if s[3].numel() > 0), key=lambda s: s[:3])
+    grads, end, last = list(grads), 0, -1
+    for begin, is_grad, i, t in spans:
+        if begin < end and is_grad:
+            grads[i] = t.clone()
+            continue
+        if begin < end and last >= 0:  # what is kept so far lies apart: the last one alone can reach this far
+            grads[last] = grads[last].clone()
+        end, last = max(end, begin + t.numel() * t.element_size()), i
+    return grads
+
+
 class AdamW(Adam):
     """tf.keras.optimizers.AdamW: ``Adam`` with decoupled weight decay, ``theta -= lr * weight_decay * theta`` ahead of the
     update, and optionally the gradients clipped by their global norm.  All variables of a model are one launch
@@ -259,7 +274,7 @@ class AdamW(Adam):
                                          for (g, v), t in zip(pairs, tv)):
             self.apply_model(pairs[0][1].owner)
             return
-        # some variables, or gradients of the caller's: a plan for this call
+        # some variables, or gradients of the caller's, which are only read and may share memory: a plan for this call
         grads = []
         for g, v in pairs:
             g = g.as_subclass(torch.Tensor).to(device=v.data.device, dtype=torch.float32).contiguous().view(-1)
@@ -267,6 +282,8 @@ class AdamW(Adam):
                 raise ValueError(f"apply_gradients: gradient of {v.name} has {g.numel()} elements, not {v.size}")
             grads.append(g)
         variables = [v for _, v in pairs]
+        owners = {id(v.owner): v.owner for v in variables}.values()
+        grads = _apart(grads, [t for m in owners for t in (m._params, *self._slots_for(m))])
         self._step(self._plan(variables, grads, False), variables[0].data.device, 1.0)
         for v in variables:
             v.owner._lp_dirty = True
