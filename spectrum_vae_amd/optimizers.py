@@ -48,6 +48,7 @@ class Adam:
         self.beta_1, self.beta_2, self.epsilon = float(beta_1), float(beta_2), float(epsilon)
         self._state: Optional[torch.Tensor] = None  # int64[3] on the device: update count, {alpha, lr}, arrival counter
         self._slots: Dict[int, Tuple[torch.Tensor, torch.Tensor]] = {}
+        self._slots_of: Dict[int, torch.Tensor] = {}  # the parameters that the slots belong to
 
     # ---- device state
     def _ensure_state(self, device):
@@ -56,11 +57,13 @@ class Adam:
         return self._state
 
     def _slots_for(self, model):
-        s = self._slots.get(id(model))
-        if s is None:
-            s = (torch.zeros_like(model._params), torch.zeros_like(model._params))
-            self._slots[id(model)] = s
-        return s
+        key = id(model)
+        if key not in self._slots or self._slots_of[key] is not model._params:  # an id is given out again once its model is gone
+            self._slots[key], self._slots_of[key] = self._zero_slots(model), model._params
+        return self._slots[key]
+
+    def _zero_slots(self, model):
+        return torch.zeros_like(model._params), torch.zeros_like(model._params)
 
     @property
     def iterations(self) -> int:
@@ -178,7 +181,7 @@ class AdamW(Adam):
         self.weight_decay = float(weight_decay)
         self.global_clipnorm = None if global_clipnorm is None else float(global_clipnorm)
         self.state_bits, self.seed = int(state_bits), int(seed)
-        self._excluded_ids, self._excluded_names = set(), ()
+        self._excluded, self._excluded_names = (), ()
         self._plans: Dict[int, tuple] = {}  # id(model) -> (model, plan)
 
     def exclude_from_weight_decay(self, var_list=None, var_names=None):
@@ -186,24 +189,20 @@ class AdamW(Adam):
         before the first step."""
         if self._plans:
             raise ValueError("exclude_from_weight_decay must be called before the first step")
-        self._excluded_ids = {id(v) for v in var_list or ()}
+        self._excluded = tuple(var_list or ())
         self._excluded_names = tuple(var_names or ())
 
     def _decay_of(self, var) -> float:
-        out = id(var) in self._excluded_ids or any(n in var.name for n in self._excluded_names)
+        out = any(var is v for v in self._excluded) or any(n in var.name for n in self._excluded_names)
         return 0.0 if out else self.weight_decay
 
     # ---- moments: flat over a model's variables; in 8 bits every variable starts on a block of its own
-    def _slots_for(self, model):
+    def _zero_slots(self, model):
         if self.state_bits == 32:
-            return super()._slots_for(model)
-        s = self._slots.get(id(model))
-        if s is None:
-            blocks = sum(-(-v.size // ops.ADAMW_BLOCK) for v in model.trainable_variables)
-            zeros = lambda n: torch.zeros(n, dtype=torch.uint8, device=model._params.device)  # noqa: E731
-            s = (zeros(blocks * ops.ADAMW_BLOCK), zeros(blocks * ops.ADAMW_BLOCK), zeros(blocks), zeros(blocks))
-            self._slots[id(model)] = s
-        return s
+            return super()._zero_slots(model)
+        blocks = sum(-(-v.size // ops.ADAMW_BLOCK) for v in model.trainable_variables)
+        zeros = lambda n: torch.zeros(n, dtype=torch.uint8, device=model._params.device)  # noqa: E731
+        return zeros(blocks * ops.ADAMW_BLOCK), zeros(blocks * ops.ADAMW_BLOCK), zeros(blocks), zeros(blocks)
 
     def _moments_of(self, var):
         """(m, v, m_exp, v_exp) of one variable; the exponents are None with 32-bit moments."""

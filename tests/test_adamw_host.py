@@ -49,3 +49,46 @@ def test_any_gradients_end_up_apart(seed):
     n, m = (int(torch.randint(1, 6, (1,), generator=g)) for _ in range(2))
     edges = sorted(torch.randint(0, 61, (2 * m,), generator=g).tolist())
     _check([cut() for _ in range(n)], [flat[i:j] for i, j in zip(edges[::2], edges[1::2])])
+
+
+class _Model:
+    """What an optimizer sees of a model."""
+
+    def __init__(self, sizes):
+        self._params = torch.zeros(sum(sizes))
+        self.trainable_variables = [type("V", (), {"size": n, "name": "v"})() for n in sizes]
+
+
+@pytest.mark.parametrize("make", ["Adam", "AdamW", "AdamW8"])
+def test_a_model_in_the_place_of_one_that_is_gone_starts_with_moments_of_its_own(make):
+    """An id is given out again once its object is gone."""
+    import gc
+
+    from spectrum_vae_amd.optimizers import Adam, AdamW
+    opt = Adam() if make == "Adam" else AdamW(state_bits=8 if make == "AdamW8" else 32)
+    for i in range(20):
+        m = _Model([300, 5 + i])
+        slots = opt._slots_for(m)
+        assert all(not t.any() for t in slots)
+        assert slots[0].numel() == (256 * 3 if make == "AdamW8" else 305 + i)
+        assert opt._slots_for(m)[0] is slots[0]
+        for t in slots:
+            t.fill_(1)
+        del m, slots
+        gc.collect()
+
+
+def test_a_variable_in_the_place_of_an_excluded_one_is_decayed():
+    import gc
+
+    from spectrum_vae_amd.optimizers import AdamW
+    opt = AdamW(weight_decay=0.1)
+
+    class V:
+        name = "kernel"
+
+    kept = V()
+    opt.exclude_from_weight_decay(var_list=[V(), kept])
+    gc.collect()
+    others = [V() for _ in range(20)]
+    assert opt._decay_of(kept) == 0.0 and all(opt._decay_of(v) == 0.1 for v in others)
