@@ -393,6 +393,11 @@ int sv_batchnorm_sync_bwd_apply(const void* x, const void* dy, const void* y_act
  *    inputs.
  *  workspace: sv_groupnorm_workspace_bytes, 16-byte aligned, for either direction. */
 size_t sv_groupnorm_workspace_bytes(int64_t N, int64_t S, int C, int groups);
+/*  sv_groupnorm_form: how a call with these extents is laid out, for tests and measurements (`alignment`: bytes that the addresses of
+ *  all tensors are a multiple of).  form[0..6] = pieces a thread holds (0: the streamed form), threads of a workgroup, elements of a
+ *  piece, whole groups summed (1) or channels (0), nontemporal stores (1) and loads (2) of the held form, slabs of channels, chunks of a
+ *  sample. */
+int sv_groupnorm_form(int64_t N, int64_t S, int C, int groups, int backward, int dtype, int alignment, int32_t* form);
 int sv_groupnorm_act_fwd(const void* x, const float* gamma, const float* beta, void* y, float* save_mean, float* save_rstd,
                          int64_t N, int64_t S, int C, int groups, float eps, int act, float alpha, void* workspace,
                          size_t workspace_bytes, int dtype, sv_stream_t stream);

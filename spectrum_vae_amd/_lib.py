@@ -145,6 +145,7 @@ SIGNATURES = {
     "sv_batchnorm_act_bwd": (_i, [_p, _p, _p, _i, _f, _p, _p, _p, _p, _p, _p, _i, _i, _f, _p, _i, _i64, _i, _i, _p, _sz,
                                   _i, _p]),
     "sv_groupnorm_workspace_bytes": (_sz, [_i64, _i64, _i, _i]),
+    "sv_groupnorm_form": (_i, [_i64, _i64, _i, _i, _i, _i, _i, C.POINTER(C.c_int32)]),
     "sv_groupnorm_act_fwd": (_i, [_p] * 6 + [_i64, _i64, _i, _i, _f, _i, _f, _p, _sz, _i, _p]),
     "sv_groupnorm_act_bwd": (_i, [_p] * 9 + [_i, _i64, _i64, _i, _i, _i, _f, _p, _sz, _i, _p]),
     "sv_concat_channels_fwd": (_i, [_p, _p, _p, _i64, _i, _i, _i, _p]),

@@ -7,7 +7,7 @@ that are not contiguous float32 on a GPU, so a silent CPU path cannot exist.
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -562,6 +562,27 @@ def groupnorm_workspace(n: int, s: int, c: int, groups: int) -> int:
     """Scratch bytes of ``groupnorm_act_fwd`` / ``groupnorm_act_bwd`` on [n, s, c] activations (s: product of the spatial
     extents)."""
     return int(lib.sv_groupnorm_workspace_bytes(n, s, c, groups))
+
+
+class GroupNormForm(NamedTuple):
+    """How a group norm call is laid out (``groupnorm_form``)."""
+
+    held: int         # pieces of a tensor that a thread holds; 0: the streamed form
+    threads: int
+    piece: int        # elements of a piece
+    whole_groups: bool
+    nontemporal: int  # 1: stores, 2: loads too
+    slabs: int
+    chunks: int
+
+
+def groupnorm_form(n: int, s: int, c: int, groups: int, backward: bool, dtype, alignment: int = 256) -> GroupNormForm:
+    """The layout of a ``groupnorm_act_fwd`` / ``_bwd`` call on [n, s, c] activations whose addresses are multiples of ``alignment``
+    bytes."""
+    out = (C.c_int32 * 7)()
+    check(lib.sv_groupnorm_form(n, s, c, groups, int(backward), BF16 if dtype is torch.bfloat16 else F32, alignment, out),
+          "sv_groupnorm_form")
+    return GroupNormForm(out[0], out[1], out[2], bool(out[3]), out[4], out[5], out[6])
 
 
 def _groupnorm_extents(x, like, gamma, beta, mean, rstd, groups: int):
