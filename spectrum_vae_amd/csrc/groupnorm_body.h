@@ -16,9 +16,10 @@
 //             forward   512 x 32x32x64 bf16     134 MB          32 us   4.2
 //             backward  1024 x 16x16x256 bf16   403 MB          83 us   4.8   (6 us of it gn_param_fold_k)
 //             forward   1 x 8x8x64 f32                         3.7 us
-//             backward  64 x 8x8x128 f32          6 MB         7.2 us   two launches
+//             backward  64 x 8x8x128 f32          6 MB         7.2 us   two launches in a row of calls; each by itself 5.9 and 3.0
 //   streamed  forward   2 x 512x512x128 bf16    268 MB          84 us   403 MB with the second reading: 4.8 TB/s
 //             backward  4 x 256x256x64 f32      201 MB          64 us   336 MB with the second reading: 5.2 TB/s
+//             forward   64 x 90x90x32 bf16       66 MB          27 us   two passes of 33 and 66 MB and their launches
 #pragma once
 #include <type_traits>
 
@@ -1023,10 +1024,11 @@ GnPlan gn_plan(int64_t N, int64_t S, int C, int G, int size, uintptr_t bits, boo
     // threads before 128-byte ones with 1024, of which a CU holds one (512 samples of 32x32x64 bf16 forward 32 against 41 us, 1024 of
     // 30x30x96 94 against 133; backward 59 against 57, 139 against 183) - but for the f32 forward pass of whole groups, of which it
     // holds two (1024 samples of 32x32x64 111 against 125 us).  Below 64 bytes a row the streamed form is faster, and where few
-    // workgroups would hold much each: it spreads them.  Fewer than 112 of 8192 pieces and more (50 samples of 40x40x48 bf16, 100
-    // workgroups, forward 16.1 against 17.5 us, backward 17.4 against 22.4; 31 of 239x5x64, 62 workgroups, 14.5 against 13.6 and
-    // 14.8 against 18.2), fewer than 48 of 4096 (8 of 32x32x64 f32, 32 workgroups, 8.9 against 9.6 and 9.5 against 11.1; with 100
-    // workgroups, 25 of 32x32x128 bf16, 16.8 against 12.3 and 17.0 against 17.8).
+    // workgroups would hold much each: it spreads them.  Fewer than 112 of 8192 pieces and more (37 samples of 31x29x90 bf16, 111
+    // workgroups, forward 12.8 against 13.1 us; 50 of 40x40x48, 100 workgroups, 16.4 against 17.5, backward 17.4 against 22.4; 31 of
+    // 239x5x64, 62 workgroups, forward the other way, 14.6 against 13.6, backward 14.8 against 18.2), fewer than 48 of 4096 (8 of
+    // 32x32x64 f32, 32 workgroups, 9.8 against 11.5 and 9.5 against 11.1; with 100 workgroups, 25 of 32x32x128 bf16, 17.3 against
+    // 12.2 and 17.0 against 17.8).
     struct Form {
         int row, K, NT;
         bool two;
@@ -1068,8 +1070,8 @@ GnPlan gn_plan(int64_t N, int64_t S, int C, int G, int size, uintptr_t bits, boo
         q.far = !whole(64) ? 0 : large && whole(128) ? 2 : 1;
         return q;
     }
-    // Sixteen rows a thread for two tensors and for narrow pieces, else eight (33 MB of bf16, 64 samples of 90x90x32: backward 35.8 us
-    // against 37.8, forward 29.0 against 27.7; 100 samples of 30x31x45 bf16 forward 17.8 against 22.2).
+    // Sixteen rows a thread for two tensors and for narrow pieces, else eight (33 MB of bf16, 64 samples of 90x90x32 with ELU: backward
+    // 35.8 us against 37.8, forward 28.2 against 27.3; 100 samples of 30x31x45 bf16 forward 16.4 against 19.8).
     plan_streamed(q, N, S, C, bwd || q.V * size < 8 ? 16 : 8);
     return q;
 }
@@ -1199,9 +1201,9 @@ int launch(const char* who, GnArgs& a, void* workspace, hipStream_t st) {
     } else {
         a.part = a.folded + a.N * 2 * a.C;
         // Whole groups in a slab and few chunks: the second pass joins the groups' values itself, which saves a launch (32 samples of
-        // 128x128x32 bf16 forward 28.2 -> 26.9 us, backward 38.1 -> 37.1; one of 18x67x10 f32 9.7 -> 9.0).  All of its workgroups read
+        // 128x128x32 bf16 forward 27.0 -> 25.2 us, backward 38.1 -> 37.1; one of 18x67x10 f32 10.0 -> 8.8).  All of its workgroups read
         // all of a sample's values: more than 10 MB in all cost more than the launch (two samples of 512x512x32 bf16, 1024 chunks
-        // each, 29.7 -> 38.3).  Backward, its first workgroups also add the channels' sums of all chunks.
+        // each, 28.5 -> 35.3).  Backward, its first workgroups also add the channels' sums of all chunks.
         if (q.slabs == 1 && a.N * q.chunks * q.chunks * a.G <= 5 << 18 && (!BWD || a.N * q.chunks <= 2048))
             a.groups = a.part + a.N * q.chunks * 2 * a.C;
         launch_streamed<T, BWD>(a, q, st);
