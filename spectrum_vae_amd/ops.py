@@ -579,6 +579,8 @@ class GroupNormForm(NamedTuple):
 def groupnorm_form(n: int, s: int, c: int, groups: int, backward: bool, dtype, alignment: int = 256) -> GroupNormForm:
     """The layout of a ``groupnorm_act_fwd`` / ``_bwd`` call on [n, s, c] activations whose addresses are multiples of ``alignment``
     bytes."""
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"groupnorm: float32 or bfloat16, not {dtype}")
     out = (C.c_int32 * 7)()
     check(lib.sv_groupnorm_form(n, s, c, groups, int(backward), BF16 if dtype is torch.bfloat16 else F32, alignment, out),
           "sv_groupnorm_form")

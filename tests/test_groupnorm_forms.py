@@ -67,6 +67,8 @@ def test_forms_of_calls_out_of_range_are_refused():
     for alignment in (0, 3, -4):
         with pytest.raises(_lib.SpectrumHipError, match="alignment"):
             ops.groupnorm_form(2, 4, 8, 2, False, torch.float32, alignment)
+    with pytest.raises(TypeError, match="float16"):
+        ops.groupnorm_form(2, 4, 8, 2, False, torch.float16)
     f = ops.groupnorm_form(2, 512 * 512, 128, 32, False, torch.bfloat16)
     assert f.held == 0 and f.chunks > 1
 
